@@ -1,5 +1,5 @@
-"""ctypes binding of libfe_paged.so, the C ABI declared in include/flexengine_amd.h and
-include/flexengine_amd_model.h.
+"""ctypes binding of libfe_paged.so, the C ABI declared in include/flexengine_amd.h,
+include/flexengine_amd_model.h and include/flexengine_amd_span.h.
 
 There is no fallback: if the library is missing, or no ROCm GPU is present when
 a kernel is called, the call raises RuntimeError.
@@ -93,6 +93,24 @@ SIGNATURES |= {
     "fe_gemm_rope": (_i, [_p, _p, _i, _p, _f, _i, _i, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p,
                           _p, _sz, _p]),
 }
+
+# include/flexengine_amd_span.h
+_WRITE4 = [_p, _p, _i64, _p, _p, _p, _p, _i]
+SIGNATURES |= {
+    "fe_write_kv4": (_i, _WRITE4 + [_p, _p, _i, _i, _i, _i, _p]),
+    "fe_write_kv4_decode": (_i, _WRITE4 + [_p, _i, _p, _i, _i, _i, _i, _p]),
+    "fe_write_kv4_ragged": (_i, _WRITE4 + [_p, _i, _p, _p, _i, _i, _i, _i, _i, _p]),
+    "fe_gather_kv4": (_i, [_p, _p, _p, _p, _i, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p]),
+    "fe_span_decode_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "fe_paged_decode_window": (_i, [_p, _i64, _p, _p, _p, _i64, _p, _p, _i, _p, _i, _p, _p, _sz,
+                                    _i, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
+    "fe_paged_decode_kv4": (_i, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i, _p, _i, _p, _p,
+                                 _sz, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
+}
+for _name in ("fe_write_kv4", "fe_write_kv4_decode", "fe_write_kv4_ragged", "fe_gather_kv4",
+              "fe_paged_decode_window", "fe_paged_decode_kv4"):
+    SIGNATURES[_name + "_bf16"] = SIGNATURES[_name]
+SIGNATURES["fe_paged_decode_window_f32"] = SIGNATURES["fe_paged_decode_window"]
 
 _LIB: ctypes.CDLL | None = None
 _LOCK = threading.Lock()

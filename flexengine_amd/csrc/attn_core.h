@@ -261,11 +261,15 @@ struct TileCore {
 // PAD: the real head_dim dr is below D (a multiple of 4): rows are dr floats
 // apart within a pool row, the dims past dr are zeros in K and V (not loaded,
 // and not written by the page write), and q is zero there too.
+//
+// SPAN: tiles span_head, span_head + 1, ... of the walk are span_skip tiles further on, and a
+// column of row tile rt sees only the keys below sinks and from wlo[rt] on (and below its
+// limit); V of the keys that no column sees (wmin: the lowest wlo) is taken as zeros.
 __device__ __forceinline__ constexpr int f32_dim0(int x, int g) {
   return 64 * (x >> 2) + 16 * g + 4 * (x & 3);
 }
 
-template <int D, bool LIST = false, bool PAD = false, int RT = 1>
+template <int D, bool LIST = false, bool PAD = false, int RT = 1, bool SPAN = false>
 struct F32Core {
   static constexpr int NC = D / 16;  // 16-byte K and q chunks per lane
   static constexpr int NW = D / 64;  // 64-dim groups of V
@@ -293,6 +297,7 @@ struct F32Core {
   // refilled every 64 tiles, so no table load sits between two tiles' loads)
   int t_first, step;
   int row_vec, list_base;
+  int span_head, span_skip, sinks, wmin, wlo[RT];  // SPAN
 
   f32x4 qv[RT][NC];
   float m_run[RT];
@@ -305,10 +310,16 @@ struct F32Core {
     const int blk = clamp_block(trow[page], NB);
     return (int64_t)blk * BS + (tok & (BS - 1));
   }
+  // first key of tile k of the wave's list
+  __device__ __forceinline__ int tile_tok(int k) const {
+    int t = t_first + k * step;
+    if constexpr (SPAN) t = t < span_head ? t : t + span_skip;
+    return t * kTile;
+  }
   // LIST: the pool rows of tiles k0 .. k0 + 63 of the wave's list
   __device__ __forceinline__ void fill_list(int k0) {
     list_base = k0;
-    row_vec = (int)pool_row((t_first + (k0 + lane_id()) * step) * kTile);
+    row_vec = (int)pool_row(tile_tok(k0 + lane_id()));
   }
   // LIST: descriptor of tile k of a pool, from its first key's row to the end of its
   // last valid key's row (loads past it return zeros)
@@ -341,7 +352,7 @@ struct F32Core {
     const int lane = lane_id();
     const int g = lane >> 4;
     const int n = lane & 15;
-    const int t0 = (t_first + k * step) * kTile;
+    const int t0 = tile_tok(k);
     if constexpr (LIST) {
       if (k - list_base >= kWave) fill_list(k);  // wave-uniform
       const __amdgpu_buffer_rsrc_t r = tile_rsrc(k_pool, k, t0);
@@ -377,7 +388,7 @@ struct F32Core {
     const int lane = lane_id();
     const int g = lane >> 4;
     const int n = lane & 15;
-    const int t0 = (t_first + k * step) * kTile;
+    const int t0 = tile_tok(k);
     if constexpr (LIST) {
       // the row step is part of the lane offset: the range check that zeroes the keys past
       // tok_end is not promised to count a scalar offset
@@ -441,13 +452,17 @@ struct F32Core {
   }
   __device__ __forceinline__ void softmax(int k, const f32x4 (&sacc)[RT], f32x4 (&p)[RT]) {
     const int g = lane_id() >> 4;
-    const int t0 = (t_first + k * step) * kTile;
+    const int t0 = tile_tok(k);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float sv[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sv[i] = t0 + 4 * g + i < limit[rt] ? sacc[rt][i] * scale_log2 : kNegInf;
+      for (int i = 0; i < 4; ++i) {
+        const int tok = t0 + 4 * g + i;
+        bool see = tok < limit[rt];
+        if constexpr (SPAN) see = see && (tok < sinks || tok >= wlo[rt]);
+        sv[i] = see ? sacc[rt][i] * scale_log2 : kNegInf;
+      }
       float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
       mx = fmaxf(mx, shfl_xor_f(mx, 16));
       mx = fmaxf(mx, shfl_xor_f(mx, 32));
@@ -465,6 +480,21 @@ struct F32Core {
       l_run[rt] += (p[rt][0] + p[rt][1]) + (p[rt][2] + p[rt][3]);
     }
   }
+  // SPAN: V of the keys of tile k that no column sees (their pages may hold anything)
+  __device__ __forceinline__ void hide(int k, f32x4 (&vv)[4][NW]) const {
+    if constexpr (SPAN) {
+      const int t0 = tile_tok(k);
+      if (t0 >= wmin || t0 + kTile <= sinks) return;  // wave-uniform
+      const int g = lane_id() >> 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = t0 + 4 * g + r;
+        if (tok >= sinks && tok < wmin)
+#pragma unroll
+          for (int w = 0; w < NW; ++w) vv[r][w] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  }
   __device__ __forceinline__ void pv(const f32x4 (&vv)[4][NW], const f32x4 (&p)[RT]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -477,10 +507,11 @@ struct F32Core {
             o[rt][4 * w + j] = mfma4_f32(vv[r][w][j], p[rt][r], o[rt][4 * w + j]);
   }
   __device__ __forceinline__ void compute_tile(int k, const f32x4 (&kk)[NC],
-                                               const f32x4 (&vv)[4][NW]) {
+                                               f32x4 (&vv)[4][NW]) {
     f32x4 sacc[RT], p[RT];
     scores(kk, sacc);
     softmax(k, sacc, p);
+    hide(k, vv);
     pv(vv, p);
   }
 
@@ -536,6 +567,7 @@ struct F32Core {
       scores(kk, sacc);
       if (k + 1 < ntiles) load_k(k + 1, kk);
       softmax(k, sacc, p);
+      hide(k, vv);
       pv(vv, p);
       if (k + 1 < ntiles) load_v(k + 1, vv);
     }

@@ -309,23 +309,30 @@ struct Piece {
 // class; the search); the lengths of the first 64 sequences are loaded once
 // and kept in registers, so a batch of up to 64 costs one round trip to
 // memory.
+//
+// walk(L): the keys of a sequence of L that are walked, all of them by default.  A kernel that
+// leaves keys out numbers the others 0 .. walk(L) - 1; tok_begin and tok_end are such numbers.
+struct WalkAll {
+  __device__ __forceinline__ int operator()(int L) const { return L; }
+};
+template <class Walk = WalkAll>
 __device__ __forceinline__ bool find_piece(const int32_t* ctx, const int32_t* tok0, int B,
                                            int max_len, int target, int item, Piece& pc,
-                                           int& total) {
+                                           int& total, Walk walk = Walk{}) {
   const int lane = lane_id();
   int L0 = 0, s0 = 0;
   if (lane < B) {
     L0 = seq_len(ctx, lane, max_len);
     s0 = suffix_start(tok0, lane, L0);
   }
-  const int nq0 = (L0 - s0 + 63) >> 6;
+  const int nq0 = (walk(L0) - s0 + 63) >> 6;
   int sum = wave_sum_i(nq0), longest = wave_max_i(nq0);
   for (int base = kWave; base < B; base += kWave) {
     const int b = base + lane;
     int nq = 0;
     if (b < B) {
       const int L = seq_len(ctx, b, max_len);
-      nq = (L - suffix_start(tok0, b, L) + 63) >> 6;
+      nq = (walk(L) - suffix_start(tok0, b, L) + 63) >> 6;
     }
     sum += wave_sum_i(nq);
     const int m = wave_max_i(nq);
@@ -351,7 +358,7 @@ __device__ __forceinline__ bool find_piece(const int32_t* ctx, const int32_t* to
       L = b < B ? seq_len(ctx, b, max_len) : 0;
       t0 = b < B ? suffix_start(tok0, b, L) : 0;
     }
-    return (L - t0 + 63) >> 6;
+    return (walk(L) - t0 + 63) >> 6;
   };
   // size class of a sequence's last piece: 0 none, 1 at least chunk/2 quads, 2 smaller
   auto rem_class = [&](int nq) __attribute__((always_inline)) {
@@ -394,7 +401,8 @@ __device__ __forceinline__ bool find_piece(const int32_t* ctx, const int32_t* to
       pc.id = readlane_i(incl_id, src) - pc.nsplit + pc.split;
       pc.tok_begin = pc.tok0 + pc.split * chunk * 64;
       const int e = pc.tok0 + (pc.split + 1) * chunk * 64;
-      pc.tok_end = e < pc.L ? e : pc.L;
+      const int end = walk(pc.L);
+      pc.tok_end = e < end ? e : end;
       return true;
     }
     carry = readlane_i(incl, kWave - 1);

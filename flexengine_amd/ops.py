@@ -12,6 +12,7 @@ import contextlib
 from dataclasses import dataclass
 import functools
 import math
+import operator
 
 import torch
 
@@ -28,6 +29,48 @@ DTYPES_16 = (FP16, BF16)
 _SFX = {FP16: "", BF16: "_bf16", FP32: "_f32"}
 # the page movers copy bytes: one form for both 16-bit types, one for fp32
 _MOVER_SFX = {FP16: "", BF16: "", FP32: "_f32"}
+
+
+@dataclass(frozen=True)
+class Kv4Pool:
+    """A K or V pool held in 4 bits (include/flexengine_amd_span.h): the functions below that
+    take pools take a pair of these in the place of two tensors.
+
+    codes uint8 [num_blocks, kv_heads, block_size, head_dim / 2], scales uint8 [num_blocks,
+    kv_heads, block_size, head_dim / 32], both with the same leading layer dim if the pool
+    holds several; dtype: the type of its rows (float16 or bfloat16).  pool[layer] is one
+    layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    dtype: torch.dtype = FP16
+
+    @classmethod
+    def empty(cls, shape, dtype: torch.dtype = FP16, device="cuda:0") -> "Kv4Pool":
+        """A pool of the plain pools' shape [..., num_blocks, block_size, kv_heads, head_dim]
+        (rows are zeros until they are written)."""
+        *lead, bs, hkv, d = shape
+        if d % 32:
+            raise ValueError("4-bit pools need a head_dim that is a multiple of 32")
+        if dtype not in DTYPES_16:
+            raise ValueError("4-bit pools hold float16 or bfloat16 rows")
+        return cls(torch.zeros((*lead, hkv, bs, d // 2), dtype=torch.uint8, device=device),
+                   torch.full((*lead, hkv, bs, d // 32), 127, dtype=torch.uint8, device=device), dtype)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        *lead, hkv, bs, half = self.codes.shape
+        return (*lead, bs, hkv, 2 * half)
+
+    @property
+    def ndim(self) -> int:
+        return self.codes.ndim
+
+    def __getitem__(self, layer: int) -> "Kv4Pool":
+        return Kv4Pool(self.codes[layer], self.scales[layer], self.dtype)
 
 
 def _require_gpu(*tensors: torch.Tensor) -> torch.device:
@@ -77,6 +120,61 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor,
     return nb, bs, hkv, d
 
 
+def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
+    if not (isinstance(k_pool, Kv4Pool) and isinstance(v_pool, Kv4Pool)):
+        raise ValueError("K and V pools must both be 4-bit pools, or both tensors")
+    if k_pool.ndim != 4 or k_pool.codes.shape != v_pool.codes.shape:
+        raise ValueError("4-bit pools must both hold one layer of [num_blocks, kv_heads, block_size]")
+    nb, hkv, bs, half = k_pool.codes.shape
+    if k_pool.dtype not in DTYPES_16 or v_pool.dtype != k_pool.dtype:
+        raise ValueError("4-bit pools must hold float16 or bfloat16 rows (both the same)")
+    for p in (k_pool, v_pool):
+        if p.codes.dtype != torch.uint8 or p.scales.dtype != torch.uint8 or half % 16 or \
+                p.scales.shape != (nb, hkv, bs, half // 16):
+            raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
+                             "[..., head_dim / 32] (head_dim a multiple of 32)")
+        if not (p.codes.is_contiguous() and p.scales.is_contiguous()):
+            raise ValueError("K/V pools must be contiguous")
+        if p.scales.device != p.codes.device:
+            raise ValueError("a 4-bit pool's codes and scales must be on one device")
+    return nb, bs, hkv, 2 * half
+
+
+def _is_kv4(k_pool, v_pool) -> bool:
+    return isinstance(k_pool, Kv4Pool) or isinstance(v_pool, Kv4Pool)
+
+
+def _any_pool(k_pool, v_pool) -> tuple[int, int, int, int]:
+    return _check_pool4(k_pool, v_pool) if _is_kv4(k_pool, v_pool) else \
+        _check_pool(k_pool, v_pool, KV_DTYPES)
+
+
+def _mover(base: str, tail: str, k_pool, v_pool) -> tuple[str, tuple]:
+    """A page mover's entry point for these pools, and the pools' pointers."""
+    if isinstance(k_pool, Kv4Pool):
+        return f"fe_{base}4{tail}{_SFX[k_pool.dtype]}", _kv4_ptrs(k_pool, v_pool)
+    return f"fe_{base}{tail}{_MOVER_SFX[k_pool.dtype]}", (k_pool.data_ptr(), v_pool.data_ptr())
+
+
+def _kv4_ptrs(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple:
+    return (k_pool.codes.data_ptr(), k_pool.scales.data_ptr(), v_pool.codes.data_ptr(),
+            v_pool.scales.data_ptr())
+
+
+def _span(window: int | None, sinks: int) -> tuple[int, int]:
+    """(window, sinks) as the library takes them (window 0: none)."""
+    sinks = operator.index(sinks)
+    if window is None:
+        if sinks:
+            raise ValueError("sinks are for a window: without one every key is seen")
+        return 0, 0
+    window = operator.index(window)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    # (a window past every context is none; the library takes 32-bit ones)
+    return min(window, 1 << 30), min(sinks, 1 << 30)
+
+
 def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise ValueError(f"{name} must be int32 (convert once with .to(torch.int32))")
@@ -91,7 +189,7 @@ def write_kv(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_p
              slot_block: torch.Tensor, slot_offset: torch.Tensor) -> None:
     """k_pool[slot_block[t], slot_offset[t]] = k_new[t] (and v); negative blocks are skipped."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, slot_block, slot_offset)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     if k_new.shape != v_new.shape or k_new.ndim != 3 or tuple(k_new.shape[1:]) != (hkv, d):
         raise ValueError("K/V shapes must be [tokens, kv_heads, head_dim]")
     if k_new.dtype != k_pool.dtype or v_new.dtype != k_pool.dtype:
@@ -102,10 +200,9 @@ def write_kv(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_p
     slot_block, slot_offset = _int32(slot_block, "slot_block"), _int32(slot_offset, "slot_offset")
     if slot_block.shape != (t,) or slot_offset.shape != (t,):
         raise ValueError("slot arrays must be [tokens]")
-    _lib.call("fe_write_kv" + _MOVER_SFX[k_pool.dtype], k_new.data_ptr(), v_new.data_ptr(),
-              k_new.stride(0),
-              k_pool.data_ptr(), v_pool.data_ptr(), nb, slot_block.data_ptr(),
-              slot_offset.data_ptr(), t, hkv, d, bs, _stream(dev))
+    name, pools = _mover("write_kv", "", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+              slot_block.data_ptr(), slot_offset.data_ptr(), t, hkv, d, bs, _stream(dev))
 
 
 def write_kv_ragged(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
@@ -115,7 +212,7 @@ def write_kv_ragged(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     rows q_offsets[s]..q_offsets[s+1]-1 are the last positions of sequence s's
     context_lens[s] tokens (the arrays prefill_paged takes; fe_write_kv_ragged)."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, block_tables, q_offsets, context_lens)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     if k_new.shape != v_new.shape or k_new.ndim != 3 or tuple(k_new.shape[1:]) != (hkv, d):
         raise ValueError("K/V shapes must be [tokens, kv_heads, head_dim]")
     if k_new.dtype != k_pool.dtype or v_new.dtype != k_pool.dtype:
@@ -127,11 +224,10 @@ def write_kv_ragged(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     s = context_lens.shape[0]
     if block_tables.ndim != 2 or block_tables.shape[0] != s or q_offsets.shape != (s + 1,):
         raise ValueError("block_tables must be [S, W], q_offsets [S+1], context_lens [S]")
-    _lib.call("fe_write_kv_ragged" + _MOVER_SFX[k_pool.dtype], k_new.data_ptr(), v_new.data_ptr(),
-              k_new.stride(0),
-              k_pool.data_ptr(), v_pool.data_ptr(), nb, block_tables.data_ptr(),
-              block_tables.shape[1], q_offsets.data_ptr(), context_lens.data_ptr(), s,
-              k_new.shape[0], hkv, d, bs, _stream(dev))
+    name, pools = _mover("write_kv", "_ragged", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+              block_tables.data_ptr(), block_tables.shape[1], q_offsets.data_ptr(),
+              context_lens.data_ptr(), s, k_new.shape[0], hkv, d, bs, _stream(dev))
 
 
 def gather_tables(mirror: torch.Tensor, row_len: torch.Tensor, rows: torch.Tensor, width: int,
@@ -189,7 +285,7 @@ def write_kv_decode(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
                     context_lens: torch.Tensor) -> None:
     """Writes row b at position context_lens[b]-1 of sequence b; rows with length 0 are skipped."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, block_tables, context_lens)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     batch = k_new.shape[0]
     if k_new.shape != v_new.shape or tuple(k_new.shape[1:]) != (hkv, d):
         raise ValueError("K/V shapes must be [batch, kv_heads, head_dim]")
@@ -201,10 +297,10 @@ def write_kv_decode(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     context_lens = _int32(context_lens, "context_lens")
     if block_tables.ndim != 2 or block_tables.shape[0] != batch or context_lens.shape != (batch,):
         raise ValueError("block_tables must be [batch, W] and context_lens [batch]")
-    _lib.call("fe_write_kv_decode" + _MOVER_SFX[k_pool.dtype], k_new.data_ptr(), v_new.data_ptr(),
-              k_new.stride(0),
-              k_pool.data_ptr(), v_pool.data_ptr(), nb, block_tables.data_ptr(),
-              block_tables.shape[1], context_lens.data_ptr(), batch, hkv, d, bs, _stream(dev))
+    name, pools = _mover("write_kv", "_decode", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+              block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(), batch, hkv,
+              d, bs, _stream(dev))
 
 
 def gather_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
@@ -212,7 +308,7 @@ def gather_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
               total_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Materialises every sequence's K/V rows: returns [total_tokens, kv_heads, head_dim] pair."""
     dev = _require_gpu(k_pool, v_pool, block_tables, context_lens, out_offsets)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     block_tables = _int32(block_tables, "block_tables")
     context_lens = _int32(context_lens, "context_lens")
     out_offsets = _int32(out_offsets, "out_offsets")
@@ -221,10 +317,10 @@ def gather_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
         raise ValueError("block_tables [batch, W], context_lens [batch], out_offsets [batch+1]")
     k_out = torch.empty((total_tokens, hkv, d), dtype=k_pool.dtype, device=dev)
     v_out = torch.empty_like(k_out)
-    _lib.call("fe_gather_kv" + _MOVER_SFX[k_pool.dtype], k_pool.data_ptr(), v_pool.data_ptr(), nb,
-              block_tables.data_ptr(),
-              block_tables.shape[1], context_lens.data_ptr(), out_offsets.data_ptr(),
-              k_out.data_ptr(), v_out.data_ptr(), batch, total_tokens, hkv, d, bs, _stream(dev))
+    name, pools = _mover("gather_kv", "", k_pool, v_pool)
+    _lib.call(name, *pools, nb, block_tables.data_ptr(), block_tables.shape[1],
+              context_lens.data_ptr(), out_offsets.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+              batch, total_tokens, hkv, d, bs, _stream(dev))
     return k_out, v_out
 
 
@@ -290,7 +386,7 @@ def decode_workspace(device: torch.device, nbytes: int, kind: str = "decode") ->
 def _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out):
     """Checks of the decode entry points; returns the normalised arguments."""
     dev = _require_gpu(q, k_pool, v_pool, block_tables, context_lens, k_new, v_new, out)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     dt = k_pool.dtype
     if q.ndim != 3 or q.shape[2] != d or q.dtype != dt:
         raise ValueError("q must be [batch, num_q_heads, head_dim] of the pools' dtype")
@@ -363,7 +459,8 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  scale: float | None = None, k_new: torch.Tensor | None = None,
                  v_new: torch.Tensor | None = None, out: torch.Tensor | None = None,
                  workspace: torch.Tensor | None = None, target_splits: int = 0,
-                 plan: DecodePlan | None = None) -> torch.Tensor:
+                 plan: DecodePlan | None = None, window: int | None = None,
+                 sinks: int = 0) -> torch.Tensor:
     """Single-token paged decode attention over one layer's pools.
 
     q [B, Hq, D] fp16, bf16 or float32, the pools' dtype (rows may be strided,
@@ -373,9 +470,32 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     context_lens-1 in the same launch.  With `plan` (paged_decode_plan on these
     block_tables / context_lens; 16-bit pools) the launch reads the partition and
     first block rows from it (fe_paged_decode_planned); same results.
+
+    window: each row attends its last `window` keys and the first `sinks` of its sequence
+    only (fe_paged_decode_window).  Pools may be Kv4Pools of q's dtype (fe_paged_decode_kv4):
+    k_new / v_new are then written in 4 bits and attended as written.  Both want block sizes
+    of at least 16, take no plan and have a workspace of their own
+    (fe_span_decode_workspace_size).
     """
     (dev, nb, bs, hkv, d, batch, hq, block_tables, context_lens, new_stride, out,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
+    kv4 = isinstance(k_pool, Kv4Pool)
+    if kv4 or window is not None or sinks:
+        window, sinks = _span(window, sinks)
+        if plan is not None:
+            raise ValueError("4-bit pools and windows take no decode plan")
+        if workspace is None:
+            workspace = decode_workspace(dev, _pure_size(
+                "fe_span_decode_workspace_size", batch, hq, hkv, d, block_tables.shape[1] * bs,
+                target_splits), kind="span_decode")
+        pools = _kv4_ptrs(k_pool, v_pool) if kv4 else (k_pool.data_ptr(), v_pool.data_ptr())
+        _lib.call(("fe_paged_decode_kv4" if kv4 else "fe_paged_decode_window") + _SFX[q.dtype],
+                  q.data_ptr(), q.stride(0), out.data_ptr(), _ptr(k_new), _ptr(v_new), new_stride,
+                  *pools, nb, block_tables.data_ptr(), block_tables.shape[1],
+                  context_lens.data_ptr(), workspace.data_ptr(),
+                  workspace.numel() * workspace.element_size(), batch, hq, hkv, d, bs,
+                  float(scale), window, sinks, int(target_splits), _stream(dev))
+        return out
     need = decode_workspace_bytes(batch, hq, d, block_tables.shape[1] * bs, target_splits)
     if workspace is None:
         workspace = decode_workspace(dev, need)
@@ -417,6 +537,8 @@ def paged_decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     the private suffixes per row, merged by log-sum-exp (fe_paged_decode_shared_prefix,
     or its _bf16 / _f32 form for bfloat16 / float32 q and pools).
     """
+    if _is_kv4(k_pool, v_pool):
+        raise ValueError("the shared-prefix decode has no form for 4-bit pools")
     (dev, nb, bs, hkv, d, batch, hq, block_tables, context_lens, new_stride, out,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
     group_offsets = _int32(group_offsets, "group_offsets")
