@@ -106,11 +106,18 @@ SIGNATURES |= {
                                     _i, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
     "fe_paged_decode_kv4": (_i, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i, _p, _i, _p, _p,
                                  _sz, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
+    "fe_span_prefill_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "fe_prefill_paged_window": (_i, [_p, _p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i,
+                                     _f, _i, _i, _p, _sz, _p]),
+    "fe_prefill_paged_kv4": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i,
+                                  _i, _f, _i, _i, _p, _sz, _p]),
 }
 for _name in ("fe_write_kv4", "fe_write_kv4_decode", "fe_write_kv4_ragged", "fe_gather_kv4",
-              "fe_paged_decode_window", "fe_paged_decode_kv4"):
+              "fe_paged_decode_window", "fe_paged_decode_kv4", "fe_prefill_paged_window",
+              "fe_prefill_paged_kv4"):
     SIGNATURES[_name + "_bf16"] = SIGNATURES[_name]
-SIGNATURES["fe_paged_decode_window_f32"] = SIGNATURES["fe_paged_decode_window"]
+for _name in ("fe_paged_decode_window", "fe_prefill_paged_window"):
+    SIGNATURES[_name + "_f32"] = SIGNATURES[_name]
 
 _LIB: ctypes.CDLL | None = None
 _LOCK = threading.Lock()

@@ -1,0 +1,694 @@
+// Ragged causal prefill under a window with sinks, and over 4-bit pools, for gfx950.
+//
+// Sequence s contributes the query rows q_off[s] .. q_off[s + 1] - 1, the last n_s positions of
+// its context; a query at position p sees the keys j <= p with p - j < window and those with
+// j < sinks (without a window every j <= p).
+//
+// Work split: for one KV head the rows of a sequence are the pairs (position, query head of the
+// group), position-major (row r: position r / G), so the G heads share what is read of K and V.
+// A unit is 32 * NW such rows of one sequence and KV head, one workgroup of NW waves of 32 rows
+// each; it walks the 64-key blocks from the first to the sinks' last and then from the one that
+// holds its first row's window start to its last row's position.  Blocks between are not read,
+// keys of an edge block that no row of the unit sees are taken as zeros (their pages may hold
+// anything).  Where the units are too few for the chip, up to KS workgroups share one, each an
+// equal run of its blocks: each writes normalised fp32 rows and base-2 log-sum-exps with
+// device-coherent stores, waits for them and draws a ticket; the last one merges and sets the
+// ticket back to zero.
+//
+// One block (lane (hf, n) = (lane / 32, lane % 32) holds row n of its wave), both products on
+// v_mfma_f32_32x32x16:
+//   S^T[32 keys x 32 rows] = K.Q^T, two key tiles; register i holds the score of key 8 (i / 4)
+//     + 4 hf + i % 4 of the tile, so a row's maximum takes one exchange between the halves;
+//   base-2 online softmax with the lazy rescale, masks only on blocks at an edge of some row;
+//   O^T[32 dims x 32 rows] += V^T.P^T: the probabilities are the B operand as they stand, two
+//     transposing LDS reads give the A operand the same keys.
+//
+// K and V of a block sit in LDS as 16-bit rows whose 16-byte chunks are XOR-swizzled (all 64
+// banks busy in both reads), two stages: while one block is computed the next arrives.  16-bit
+// pools come by LDS DMA (buffer_load ... lds), one 8- or 16-key run a wave.  4-bit pools come
+// through registers: a thread loads 16-byte chunks -- 32 codes, one block with one scale --
+// two key blocks ahead, and converts them (16 conversions and four 16-byte LDS writes a chunk)
+// one block ahead; at D = 128 and NW = 8 that is one chunk a thread and block, beside the 48
+// matrix instructions of its wave.
+#pragma once
+
+#include "kv4.h"
+#include "flexengine_amd_span.h"
+
+namespace fe {
+namespace {
+
+constexpr int kSpanKeys = 64;      // keys per staged block
+constexpr int kSpanMaxSplits = 16;
+constexpr int kSpanTickets = 65536;
+constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
+constexpr int kSpanSc1 = 16;       // buffer-instruction cache policy: sc1 (device-coherent)
+// Blocks of a walk over which the reference of the softmax follows every block's maximum in
+// either direction (the probabilities' rounding is then relative to the block's own largest),
+// and the slack of the lazy rescale after them
+constexpr int kSpanFollow = 2;
+constexpr float kSpanSlack = 2.f;
+
+struct SpanPrefill {
+  const f16* q;
+  f16* out;
+  const void* k_pool;  // 4-bit: codes
+  const void* v_pool;
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  const int32_t* tables;
+  const int32_t* q_off;
+  const int32_t* ctx;
+  float* part_o;    // [KS][total_q * Hq][D]
+  float* part_lse;  // [KS][total_q * Hq]
+  int* tickets;     // [units bound][Hkv], zero between calls
+  int W, S, total_q, Hq, Hkv, G, BS, bs_log2, NB, KS;
+  int split_blocks;  // key blocks a split has at least
+  int dr;            // the real head_dim (PAD: below D)
+  float scale_log2;
+  Span span;
+};
+
+// A unit of work: rows r0 .. r0 + ROWS - 1 (fewer at the end) of sequence s
+struct SpanUnit {
+  int s, block, n, q0, ctx;
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUnit& u) {
+  const int lane = lane_id();
+  int carry = 0;
+  for (int base = 0; base < a.S; base += kWave) {
+    const int s = base + lane < a.S ? base + lane : a.S - 1;
+    const int e0 = a.q_off[s], e1 = a.q_off[s + 1], cx = clamp_len(a.ctx[s]);
+    // rows outside [0, total_q) are dropped
+    const int q0 = min(max(e0, 0), a.total_q);
+    const int n = base + lane < a.S ? max(min(e1, a.total_q) - q0, 0) : 0;
+    const int nb = (int)(((int64_t)n * a.G + ROWS - 1) / ROWS);
+    const int incl = wave_scan_incl_i(nb) + carry;
+    const unsigned long long hit = __ballot(item >= incl - nb && item < incl);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      u.s = base + src;
+      u.block = item - readlane_i(incl - nb, src);
+      u.n = readlane_i(n, src);
+      u.q0 = readlane_i(q0, src);
+      u.ctx = readlane_i(cx, src);
+      return true;
+    }
+    carry = readlane_i(incl, kWave - 1);
+  }
+  return false;
+}
+
+template <int D>
+struct SpanCfg {
+  static constexpr int ROWB = D * 2;                // LDS bytes per staged key row
+  static constexpr int MAT = kSpanKeys * ROWB;
+  static constexpr int CPR = D / 8;                 // 16-byte chunks per row
+  static constexpr int RPI = kWave / CPR;           // rows per DMA instruction
+  // chunk swizzles of row r (K: 32 rows read one chunk each; V: 4 rows x 64 bytes)
+  static __device__ __forceinline__ int swz_k(int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); }
+  static __device__ __forceinline__ int swz_v(int r) {
+    return D >= 128 ? ((r & 3) << 2) : (((r >> 1) & 1) << 2);
+  }
+};
+
+__device__ __forceinline__ float span_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float other_half(float x, int hf) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(hf ? b[0] : b[1]);
+}
+
+typedef __attribute__((address_space(3))) void span_lds_void;
+typedef __attribute__((address_space(3))) s16x4 span_lds_s16x4;
+typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)addr);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(addr >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
+                                           (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
+// The state of a wave's 32 rows
+template <int D>
+struct SpanRows {
+  f16x8 qv[D / 16];
+  int pos, lo;  // the lane's row sees keys lo .. pos (and those below the sinks)
+  float m, l;   // running reference (base 2) and this lane's part of the sum
+  f32x16 o[D / 32];
+};
+
+// One staged block whose first key is t0.  mask: some row does not see all of it.
+template <int D, class E>
+__device__ __forceinline__ void span_block(int t0, const unsigned char* kst, const unsigned char* vst,
+                                           bool mask, int sinks, float scale_log2, bool follow,
+                                           SpanRows<D>& r) {
+  using C = SpanCfg<D>;
+  constexpr int NC = D / 16, NT = D / 32;
+  const int lane = lane_id();
+  const int hf = lane >> 5;
+  const int n = lane & 31;
+  f16x8 kf[2][NC];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      kf[kt][c] = *reinterpret_cast<const f16x8*>(kst + (32 * kt + n) * C::ROWB +
+                                                  (((2 * c + hf) ^ C::swz_k(n)) * 16));
+  f32x16 st[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) st[kt] = f32x16{};
+  // all reads ahead of the MFMAs: the scheduler would interleave them to save registers, and
+  // each MFMA would wait for its read (D = 256 has no registers for that: 420 bytes of scratch)
+  if constexpr (D <= 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) st[kt] = mma32x32<E>(kf[kt][c], r.qv[c], st[kt]);
+  const int l16 = lane & 15;
+  const int vrow = 4 * hf + (l16 >> 2);
+  const int vchunk = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+  const int vswz = C::swz_v(vrow);
+  auto vfrag = [&](int s, int x) __attribute__((always_inline)) {
+    const unsigned char* vb = vst + (16 * s + vrow) * C::ROWB + (l16 & 1) * 8;
+    const int slot = ((4 * x + vchunk) ^ vswz) * 16;
+    const f16x4 a = __builtin_bit_cast(
+        f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((span_lds_s16x4*)(vb + slot)));
+    const f16x4 b = __builtin_bit_cast(
+        f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((span_lds_s16x4*)(vb + 8 * C::ROWB + slot)));
+    return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  };
+  // the first 32 keys' V fragments are read before the softmax, which hides their latency
+  f16x8 vf[2][NT];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int x = 0; x < NT; ++x) vf[s][x] = vfrag(s, x);
+
+  if (mask) {  // wave-uniform
+    int past = r.pos - t0 - 4 * hf, before = r.lo - t0 - 4 * hf, sink = sinks - t0 - 4 * hf;
+    // (defined here as far as the compiler knows: otherwise it hoists the comparisons out of
+    // the branch)
+    asm volatile("" : "+v"(past), "+v"(before), "+v"(sink));
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = 32 * kt + 8 * (i / 4) + i % 4;
+        if (key > past || (key < before && key >= sink)) st[kt][i] = kNegInf;
+      }
+  }
+  float mx = st[0][0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) mx = span_max(mx, st[0][i]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx = span_max(mx, st[1][i]);
+  mx = span_max(mx, other_half(mx, hf)) * scale_log2;
+  if (__ballot(mx > r.m + (follow ? kNegInf : kSpanSlack))) {  // wave-uniform
+    float m_new = fmaxf(r.m, mx);
+    if (follow) {
+      // down to the block's maximum too, as long as the sum stays below 2^16 of its largest
+      const float l = r.l + other_half(r.l, hf);
+      m_new = fmaxf(mx, r.m - fmaxf(16.f - __builtin_amdgcn_logf(l), 0.f));
+    }
+    const float alpha = m_new == kNegInf ? 1.f : exp2_fast(r.m - m_new);
+    r.l *= alpha;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) r.o[x] *= alpha;
+    r.m = m_new;
+  }
+  const float neg_m = r.m == kNegInf ? 0.f : -r.m;
+  f16x8 pb[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    // probabilities in 16 bits for the matrix instruction; the sum takes the rounded ones
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      pb[s][j] = to16<E>(exp2_fast(__builtin_fmaf(st[s / 2][8 * (s % 2) + j], scale_log2, neg_m)));
+    r.l = sum8<E>(pb[s], r.l);
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const f16x8 va = vf[s % 2][x];
+      if (s < 2) vf[s][x] = vfrag(s + 2, x);  // in flight during the next 16 keys' products
+      r.o[x] = mma32x32<E>(va, pb[s], r.o[x]);
+    }
+}
+
+// What a unit reads: the blocks of its walk, and which keys any of its rows sees
+struct SpanWalk {
+  int head, skip;        // blocks head, head + 1, ... of the walk are `skip` blocks further on
+  int key_end, ws, sinks;
+  __device__ __forceinline__ int block(int j) const { return j < head ? j : j + skip; }
+  __device__ __forceinline__ bool sees(int key) const {
+    return key < key_end && (key < sinks || key >= ws);
+  }
+  // every key of t0 .. t0 + n - 1
+  __device__ __forceinline__ bool sees_all(int t0, int n) const {
+    return t0 + n <= key_end && (t0 >= ws || t0 + n <= sinks);
+  }
+};
+
+// 16-bit pools: wave w brings keys RUN w .. +RUN of a block by LDS DMA
+template <int D, bool PAD, int NW>
+struct Stage16 {
+  using C = SpanCfg<D>;
+  static constexpr int RUN = kSpanKeys / NW;
+  static constexpr int NI = RUN / C::RPI;
+  static_assert(RUN <= 16 && NI >= 1, "a run lies in one page");
+  int w, id_base;
+  int idv;              // lane j: pool block of this wave's run of walk block id_base + j
+  uint32_t vk[NI], vv[NI];  // lane offsets of the DMA, the swizzles applied
+
+  __device__ __forceinline__ void load_ids(const SpanPrefill& a, const SpanWalk& wk,
+                                           const int32_t* trow, int base) {
+    id_base = base;
+    int page = (wk.block(base + lane_id()) * kSpanKeys + RUN * w) >> a.bs_log2;
+    page = page < a.W ? page : a.W - 1;
+    idv = trow[page];
+  }
+  __device__ __forceinline__ void init(const SpanPrefill& a, const SpanWalk& wk,
+                                       const int32_t* trow, int h, int j0) {
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    load_ids(a, wk, trow, j0);
+    const int rs = a.Hkv * a.dr * 2;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int rr = C::RPI * i + lane_id() / C::CPR;
+      const int sl = lane_id() % C::CPR;
+      const int ck = sl ^ C::swz_k(RUN * w + rr), cv = sl ^ C::swz_v(RUN * w + rr);
+      // chunks past the real row come from past the descriptor's end: zeros
+      vk[i] = !PAD || ck * 8 < a.dr ? (uint32_t)(rr * rs + ck * 16) : 0x7ffffff0u;
+      vv[i] = !PAD || cv * 8 < a.dr ? (uint32_t)(rr * rs + cv * 16) : 0x7ffffff0u;
+    }
+  }
+  __device__ __forceinline__ void fetch(const SpanPrefill& a, const SpanWalk& wk,
+                                        const int32_t* trow, int h, int j, unsigned char* kst,
+                                        unsigned char* vst) {
+    if (j - id_base >= kWave) {  // wave-uniform
+      load_ids(a, wk, trow, j);
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    }
+    const int t0 = wk.block(j) * kSpanKeys + RUN * w;
+    const int id = clamp_block(__builtin_amdgcn_readlane(idv, j - id_base), a.NB);
+    const int rs = a.Hkv * a.dr * 2;
+    int nv = wk.key_end - t0;
+    nv = nv < 0 ? 0 : (nv > RUN ? RUN : nv);
+    const uint32_t bytes = nv > 0 ? (uint32_t)((nv - 1) * rs + a.dr * 2) : 0u;
+    const int64_t off =
+        (((int64_t)id * a.BS + (t0 & (a.BS - 1))) * a.Hkv + h) * (int64_t)a.dr;
+    const __amdgpu_buffer_rsrc_t rk = span_rsrc((const f16*)a.k_pool + off, bytes);
+    const __amdgpu_buffer_rsrc_t rv = span_rsrc((const f16*)a.v_pool + off, bytes);
+    const bool edge = !(t0 >= wk.ws || t0 + RUN <= wk.sinks);  // wave-uniform
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t ok = vk[i], ov = vv[i];
+      if (edge && !wk.sees(t0 + C::RPI * i + lane_id() / C::CPR)) ok = ov = 0x7ffffff0u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rk, (span_lds_void*)(kst + (RUN * w + i * C::RPI) * C::ROWB), 16, ok, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rv, (span_lds_void*)(vst + (RUN * w + i * C::RPI) * C::ROWB), 16, ov, 0, 0, 0);
+    }
+  }
+};
+
+// 4-bit pools: a thread's chunks of a block, loaded into registers and converted into LDS
+template <int D, class E, bool PAD, int NW>
+struct Stage4 {
+  using C = SpanCfg<D>;
+  static constexpr int T = NW * kWave;
+  static constexpr int BPR = D / kQ4Block;                 // chunks (32 dims) per row
+  static constexpr int CHUNKS = 2 * kSpanKeys * BPR;       // of a block: K's, then V's
+  static constexpr int NI = (CHUNKS + T - 1) / T;
+  span_u32x4 codes[NI];
+  uint32_t scale[NI];
+  int id[NI];
+
+  static __device__ __forceinline__ int chunk(int i) { return threadIdx.x + i * T; }
+  static __device__ __forceinline__ int key_of(int i) { return chunk(i) / BPR % kSpanKeys; }
+  __device__ __forceinline__ void load_ids(const SpanPrefill& a, const SpanWalk& wk,
+                                           const int32_t* trow, int j) {
+    const int t0 = wk.block(j) * kSpanKeys;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      int page = (t0 + key_of(i)) >> a.bs_log2;
+      page = page < a.W ? page : a.W - 1;
+      id[i] = trow[page];
+    }
+  }
+  __device__ __forceinline__ void load(const SpanPrefill& a, const SpanWalk& wk, int h, int j) {
+    const int t0 = wk.block(j) * kSpanKeys;
+    const int cb = a.dr / 2, sb = a.dr / kQ4Block;
+    const bool all = wk.sees_all(t0, kSpanKeys);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = chunk(i), key = t0 + key_of(i), blk = c % BPR;
+      const bool is_v = c >= kSpanKeys * BPR;
+      codes[i] = span_u32x4{0, 0, 0, 0};
+      scale[i] = kQ4ScaleLow;
+      if (c < CHUNKS && (!PAD || blk < sb) && (all || wk.sees(key))) {
+        const int64_t row =
+            ((int64_t)clamp_block(id[i], a.NB) * a.Hkv + h) * a.BS + (key & (a.BS - 1));
+        const uint8_t* cp = (const uint8_t*)(is_v ? a.v_pool : a.k_pool);
+        const uint8_t* sp = is_v ? a.v_scales : a.k_scales;
+        codes[i] = *reinterpret_cast<const span_u32x4*>(cp + row * cb + blk * 16);
+        scale[i] = sp[row * sb + blk];
+      }
+    }
+  }
+  __device__ __forceinline__ void put(unsigned char* kst, unsigned char* vst) const {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = chunk(i), key = key_of(i), blk = c % BPR;
+      if (CHUNKS % T != 0 && c >= CHUNKS) continue;
+      const bool is_v = c >= kSpanKeys * BPR;
+      unsigned char* row = (is_v ? vst : kst) + key * C::ROWB;
+      const int swz = is_v ? C::swz_v(key) : C::swz_k(key);
+      const float s = q4_scale_value(scale[i]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f16x8*>(row + ((4 * blk + q) ^ swz) * 16) = q4_unpack8<E>(codes[i][q], s);
+    }
+  }
+};
+
+template <int D, class E, bool Q4, bool PAD, int NW>
+__global__ __launch_bounds__(NW* kWave)
+__attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2, D > 128 ? 1 : 2)))
+void span_prefill_kernel(const SpanPrefill a) {
+  using C = SpanCfg<D>;
+  constexpr int ROWS = 32 * NW;
+  // one LDS object per stage and matrix: the compiler's wait for an LDS DMA before an LDS read
+  // is then limited to reads of the object it fills
+  __shared__ __align__(16) unsigned char k0[C::MAT];
+  __shared__ __align__(16) unsigned char v0[C::MAT];
+  __shared__ __align__(16) unsigned char k1[C::MAT];
+  __shared__ __align__(16) unsigned char v1[C::MAT];
+  __shared__ int last;
+  // workgroup i: (KV head, key split) pair i % (Hkv KS), the later units, which see more keys,
+  // first
+  const int pairs = a.Hkv * a.KS;
+  const int items = (int)gridDim.x / pairs;
+  const int item = items - 1 - (int)blockIdx.x / pairs;
+  const int h = (int)blockIdx.x % pairs % a.Hkv;
+  const int ks = (int)blockIdx.x % pairs / a.Hkv;
+  SpanUnit u;
+  if (!find_unit<ROWS>(a, item, u)) return;
+  const int G = a.G;
+  const int DR = PAD ? a.dr : D;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = lane_id();
+  const int hf = lane >> 5;
+  const int n = lane & 31;
+  const int ctx = min(u.ctx, a.W * a.BS);
+  const int total_rows = u.n * G;
+  const int cached = ctx >= u.n ? ctx - u.n : 0;
+  const int r0 = u.block * ROWS;
+  const int r_last = min(r0 + ROWS, total_rows) - 1;
+
+  SpanWalk wk;
+  wk.key_end = cached + r_last / G + 1;
+  wk.sinks = a.span.sinks;
+  wk.ws = window_start(a.span, cached + r0 / G);
+  wk.head = (int)(((unsigned)wk.sinks + kSpanKeys - 1) / kSpanKeys);
+  wk.skip = span_skip(a.span, wk.ws, kSpanKeys);
+  const int nb = (wk.key_end + kSpanKeys - 1) / kSpanKeys - wk.skip;
+  // splits of this unit: no shorter than split_blocks
+  int splits = nb / a.split_blocks;
+  splits = splits < 1 ? 1 : (splits > a.KS ? a.KS : splits);
+  if (ks >= splits) return;
+  const int j0 = (int)((int64_t)nb * ks / splits), j1 = (int)((int64_t)nb * (ks + 1) / splits);
+
+  const int wr0 = r0 + 32 * w;
+  const bool has_rows = wr0 <= r_last;
+  // positions of the wave's first and last row, and where their windows start
+  const int p_first = cached + min(wr0, r_last) / G, p_last = cached + min(wr0 + 31, r_last) / G;
+  const int lo_first = window_start(a.span, p_first), lo_last = window_start(a.span, p_last);
+  const int row = wr0 + n;
+  const bool valid = row < total_rows;
+  const int rc = valid ? row : r_last;
+  const int32_t* trow = a.tables + (int64_t)u.s * a.W;
+  SpanRows<D> r;
+  r.pos = cached + rc / G;
+  r.lo = window_start(a.span, r.pos);
+  r.m = kNegInf;
+  r.l = 0.f;
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x) r.o[x] = f32x16{};
+  {
+    const f16* qrow = a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR + 8 * hf;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      r.qv[c] = valid && (!PAD || 16 * c + 8 * hf < DR) ? ld16(qrow + 16 * c) : f16x8{};
+  }
+  auto compute = [&](int j, const unsigned char* kst, const unsigned char* vst)
+                     __attribute__((always_inline)) {
+    const int t0 = wk.block(j) * kSpanKeys;
+    const bool sink = t0 + kSpanKeys <= wk.sinks;
+    if (!has_rows || t0 > p_last || (t0 + kSpanKeys <= lo_first && t0 >= wk.sinks)) return;
+    const bool mask = t0 + kSpanKeys - 1 > p_first || (t0 < lo_last && !sink);
+    span_block<D, E>(t0, kst, vst, mask, wk.sinks, a.scale_log2, j - j0 < kSpanFollow, r);
+  };
+
+  if constexpr (Q4) {
+    Stage4<D, E, PAD, NW> st;
+    st.load_ids(a, wk, trow, j0);
+    st.load(a, wk, h, j0);
+    if (j0 + 1 < j1) st.load_ids(a, wk, trow, j0 + 1);
+    st.put(k0, v0);
+    if (j0 + 1 < j1) st.load(a, wk, h, j0 + 1);
+    if (j0 + 2 < j1) st.load_ids(a, wk, trow, j0 + 2);
+    // step j: block j is staged once every wave has passed the barrier, and no wave reads block
+    // j - 1 any more, whose stage block j + 1 goes into
+    auto step = [&](int j, unsigned char* kc, unsigned char* vc, unsigned char* kn,
+                    unsigned char* vn) __attribute__((always_inline)) {
+      __syncthreads();
+      if (j + 1 < j1) st.put(kn, vn);
+      if (j + 2 < j1) st.load(a, wk, h, j + 2);
+      if (j + 3 < j1) st.load_ids(a, wk, trow, j + 3);
+      compute(j, kc, vc);
+    };
+    for (int j = j0; j < j1; j += 2) {
+      step(j, k0, v0, k1, v1);
+      if (j + 1 < j1) step(j + 1, k1, v1, k0, v0);
+    }
+  } else {
+    Stage16<D, PAD, NW> st;
+    st.init(a, wk, trow, h, j0);
+    st.fetch(a, wk, trow, h, j0, k0, v0);
+    auto step = [&](int j, unsigned char* kc, unsigned char* vc, unsigned char* kn,
+                    unsigned char* vn) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's run of block j is in LDS
+      __syncthreads();
+      if (j + 1 < j1) st.fetch(a, wk, trow, h, j + 1, kn, vn);
+      compute(j, kc, vc);
+    };
+    for (int j = j0; j < j1; j += 2) {
+      step(j, k0, v0, k1, v1);
+      if (j + 1 < j1) step(j + 1, k1, v1, k0, v0);
+    }
+  }
+
+  const float l = r.l + other_half(r.l, hf);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (splits == 1) {
+    if (!valid) return;
+    f16* orow = a.out + ((int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G) * DR + 4 * hf;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 t = {r.o[x][4 * q4], r.o[x][4 * q4 + 1], r.o[x][4 * q4 + 2], r.o[x][4 * q4 + 3]};
+        if (!PAD || 32 * x + 8 * q4 + 4 * hf < DR)
+          *reinterpret_cast<f16x4*>(orow + 32 * x + 8 * q4) = to16x4<E>(t * inv);
+      }
+    return;
+  }
+
+  // ---- the split's rows, and the join by the unit's last split (the host keeps the partials
+  // under 2 GiB) ----
+  const int64_t split_rows = (int64_t)a.total_q * a.Hq;
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+      a.part_o, 0, (int)(a.KS * split_rows * D * 4), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(
+      a.part_lse, 0, (int)(a.KS * split_rows * 4), 0x00020000);
+  if (valid) {
+    const uint32_t prow = (uint32_t)(ks * split_rows + (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 t = {r.o[x][4 * q4], r.o[x][4 * q4 + 1], r.o[x][4 * q4 + 2], r.o[x][4 * q4 + 3]};
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(span_u32x4, t * inv), ro,
+            (prow * D + 32 * x + 8 * q4 + 4 * hf) * (uint32_t)sizeof(float), 0, kSpanSc1);
+      }
+    if (hf == 0)
+      __builtin_amdgcn_raw_buffer_store_b32(
+          __builtin_bit_cast(uint32_t, l > 0.f ? r.m + log2f(l) : kNegInf), rl,
+          prow * (uint32_t)sizeof(float), 0, kSpanSc1);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows are complete
+  __syncthreads();
+  int* const ticket = a.tickets + item * a.Hkv + h;
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           splits - 1;
+  __syncthreads();
+  if (!last) return;
+  if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // thread -> (row, 4 dims); four splits read in one round trip
+  constexpr int TPR = D / 4;
+  const int d4 = (int)(threadIdx.x % TPR) * 4;
+  for (int row = r0 + (int)threadIdx.x / TPR; row <= r_last; row += NW * kWave / TPR) {
+    const int64_t orow = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
+    float M = kNegInf, den = 0.f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+      float lv[4];
+      f32x4 ov[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int s = s0 + k < splits ? s0 + k : splits - 1;
+        const uint32_t prow = (uint32_t)(s * split_rows + orow);
+        lv[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                              rl, prow * (uint32_t)sizeof(float), 0, kSpanSc1));
+        ov[k] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       ro, (prow * D + d4) * (uint32_t)sizeof(float), 0, kSpanSc1));
+      }
+      float bm = M;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (s0 + k >= splits) lv[k] = kNegInf;
+        bm = fmaxf(bm, lv[k]);
+      }
+      const float alpha = M == kNegInf ? 0.f : exp2f(M - bm);
+      num *= alpha;
+      den *= alpha;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float wt = lv[k] == kNegInf ? 0.f : exp2f(lv[k] - bm);
+        num += wt * ov[k];
+        den += wt;
+      }
+      M = bm;
+    }
+    if (!PAD || d4 < DR)
+      *reinterpret_cast<f16x4*>(a.out + orow * DR + d4) = to16x4<E>(num * (den > 0.f ? 1.f / den : 0.f));
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+inline size_t span_align(size_t x) { return (x + 255) & ~size_t(255); }
+inline int span_log2(int x) {
+  if (x <= 0 || (x & (x - 1))) return -1;
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+inline int span_dim(int d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
+
+// Launch shape, from what the host knows
+struct SpanShape {
+  int waves;  // per workgroup
+  int64_t units;
+  int ks;
+  size_t o, lse, bytes;  // workspace
+};
+inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d) {
+  SpanShape p;
+  const int64_t rows = (int64_t)total_q * (hq / hkv);
+  p.waves = 4;
+  p.units = (rows + 32 * p.waves - 1) / (32 * p.waves) + num_seqs;
+  // key splits so that about 512 workgroups run, two per CU
+  const int64_t wgs = ((rows + 32 * p.waves - 1) / (32 * p.waves)) * hkv;
+  int64_t ks = wgs > 0 ? 512 / wgs : 1;
+  ks = ks < 1 ? 1 : (ks > kSpanMaxSplits ? kSpanMaxSplits : ks);
+  if (p.units * hkv > kSpanTickets) ks = 1;
+  const int64_t part_rows = (int64_t)total_q * hq;
+  while (ks > 1 && ks * part_rows * span_dim(d) * (int64_t)sizeof(float) >= ((int64_t)1 << 31)) --ks;
+  p.ks = (int)ks;
+  p.o = kSpanTicketBytes;
+  p.lse = p.o + (ks > 1 ? span_align((size_t)ks * part_rows * span_dim(d) * sizeof(float)) : 0);
+  p.bytes = p.lse + (ks > 1 ? span_align((size_t)ks * part_rows * sizeof(float)) : 0);
+  return p;
+}
+
+template <int D, class E, bool Q4, bool PAD>
+int span_launch(const SpanPrefill& a, const SpanShape& p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.units * a.Hkv * a.KS));
+  hipLaunchKernelGGL((span_prefill_kernel<D, E, Q4, PAD, 4>), grid, dim3(4 * kWave), 0, s, a);
+  return FE_LAUNCH_STATUS();
+}
+
+// Checks and launch that the 16-bit and the 4-bit forms share
+template <class E, bool Q4>
+int span_prefill(const void* q, void* out, const void* k_pool, const void* k_scales,
+                 const void* v_pool, const void* v_scales, int num_blocks, const int32_t* tables,
+                 int table_stride, const int32_t* q_off, const int32_t* ctx, int num_seqs,
+                 int total_q, int hq, int hkv, int d, int bs, float scale, int window, int sinks,
+                 void* workspace, size_t workspace_bytes, fe_stream_t stream) {
+  FE_CHECK_ARG(num_seqs >= 0 && total_q >= 0 && hq > 0 && hkv > 0 && d > 0 && num_blocks > 0 &&
+               table_stride > 0 && window >= 0 && sinks >= 0 && hq % hkv == 0);
+  FE_CHECK_ARG(Q4 || window > 0);
+  FE_CHECK_ARG(scale > 0.f);  // the row maxima are taken on unscaled scores
+  const int bs_log2 = span_log2(bs);
+  if (bs_log2 < 0 || bs % kTile != 0) return FE_ERR_UNSUPPORTED;
+  if (d > 256 || d % (Q4 ? kQ4Block : 8) != 0) return FE_ERR_UNSUPPORTED;
+  // key positions, pool rows and the offsets within a run of keys are 32-bit in the kernel
+  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) ||
+      (int64_t)num_blocks * bs >= ((int64_t)1 << 31) || (int64_t)hkv * d >= ((int64_t)1 << 25) ||
+      (int64_t)total_q * (hq / hkv) >= ((int64_t)1 << 30))
+    return FE_ERR_UNSUPPORTED;
+  if (num_seqs == 0 || total_q == 0) return FE_OK;
+  FE_CHECK_ARG(q && out && k_pool && v_pool && tables && q_off && ctx);
+  if (Q4) FE_CHECK_ARG(k_scales && v_scales);
+  const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
+  const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d);
+  if (p.units * hkv * p.ks >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
+  if (workspace == nullptr || workspace_bytes < p.bytes || !aligned(workspace))
+    return FE_ERR_WORKSPACE;
+  SpanPrefill a{};
+  a.q = (const f16*)q;
+  a.out = (f16*)out;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.k_scales = (const uint8_t*)k_scales;
+  a.v_scales = (const uint8_t*)v_scales;
+  a.tables = tables;
+  a.q_off = q_off;
+  a.ctx = ctx;
+  a.tickets = (int*)workspace;
+  a.part_o = (float*)((char*)workspace + p.o);
+  a.part_lse = (float*)((char*)workspace + p.lse);
+  a.W = table_stride;
+  a.S = num_seqs;
+  a.total_q = total_q;
+  a.Hq = hq;
+  a.Hkv = hkv;
+  a.G = hq / hkv;
+  a.BS = bs;
+  a.bs_log2 = bs_log2;
+  a.NB = num_blocks;
+  a.KS = p.ks;
+  a.split_blocks = 4;
+  a.dr = d;
+  a.scale_log2 = scale * kLog2e;
+  a.span = Span{window, window > 0 ? sinks : 0};
+  const hipStream_t s = (hipStream_t)stream;
+  if (d == 64) return span_launch<64, E, Q4, false>(a, p, s);
+  if (d == 128) return span_launch<128, E, Q4, false>(a, p, s);
+  if (d < 64) return span_launch<64, E, Q4, true>(a, p, s);
+  if (d < 128) return span_launch<128, E, Q4, true>(a, p, s);
+  return span_launch<256, E, Q4, true>(a, p, s);
+}
+
+}  // namespace
+}  // namespace fe

@@ -1,0 +1,224 @@
+// Ragged prefill under a window with sinks over fp16, bf16 and fp32 pools.
+#include "span_prefill.h"
+
+using namespace fe;
+
+namespace {
+
+// ---- fp32 pools ---------------------------------------------------------------------------
+// The plain fp32 prefill's organisation on the same engine (F32Core, attn_core.h): a workgroup
+// takes 16 * RT rows of a sequence and KV head, its four waves the row block's 16-key tiles in
+// turn -- the tiles of the sinks and those from the first row's window start on -- and the
+// waves' states are joined in LDS.  Bound by the fp32 MFMAs (154 TFLOP/s in a large product).
+constexpr int kF32Waves = 4;
+
+template <int D, int RT>
+struct SpanF32Lds {
+  static constexpr int NX = D / 16;
+  static constexpr size_t park = 0;  // [kF32Waves][RT * NX][64] x 16 bytes
+  static constexpr size_t park_m = park + (size_t)kF32Waves * RT * NX * kWave * 16;
+  static constexpr size_t park_l = park_m + (size_t)kF32Waves * RT * kWave * sizeof(float);
+  static constexpr size_t bytes = park_l + (size_t)kF32Waves * RT * kWave * sizeof(float);
+};
+
+template <int D, bool PAD, int RT>
+__global__ __launch_bounds__(kF32Waves* kWave)
+__attribute__((amdgpu_waves_per_eu(RT == 1 ? 3 : 2, 8)))
+void span_prefill_f32_kernel(const SpanPrefill a) {
+  using Core = F32Core<D, true, PAD, RT, true>;
+  using Lds = SpanF32Lds<D, RT>;
+  constexpr int ROWS = 16 * RT;
+  constexpr int NX = Core::NX;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int DR = PAD ? a.dr : D;
+  const int h = blockIdx.x % a.Hkv;
+  const int item = (int)gridDim.x / a.Hkv - 1 - (int)blockIdx.x / a.Hkv;
+  SpanUnit u;
+  if (!find_unit<ROWS>(a, item, u)) return;
+  const int G = a.G;
+  const int lane = lane_id();
+  const int g = lane >> 4;
+  const int n = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ctx = min(u.ctx, a.W * a.BS);
+  const int total_rows = u.n * G;
+  const int cached = ctx >= u.n ? ctx - u.n : 0;
+  const int r0 = u.block * ROWS;
+  const int r_last = min(r0 + ROWS, total_rows) - 1;
+
+  Core core;
+  core.k_pool = (const float*)a.k_pool;
+  core.v_pool = (const float*)a.v_pool;
+  core.k_pool_w = nullptr;
+  core.v_pool_w = nullptr;
+  core.trow = a.tables + (int64_t)u.s * a.W;
+  core.rs = (int64_t)a.Hkv * DR;
+  core.hoff = h * DR;
+  core.dr = DR;
+  core.W = a.W;
+  core.NB = a.NB;
+  core.BS = a.BS;
+  core.bs_log2 = a.bs_log2;
+  core.tok_end = cached + r_last / G + 1;
+  core.scale_log2 = a.scale_log2;
+  core.knew_row = nullptr;
+  core.vnew_row = nullptr;
+  core.new_pos = -1;
+  core.sinks = a.span.sinks;
+  core.wmin = window_start(a.span, cached + r0 / G);
+  core.span_head = (int)(((unsigned)a.span.sinks + kTile - 1) / kTile);
+  core.span_skip = span_skip(a.span, core.wmin, kTile);
+  const int ntiles =
+      core.begin(w, kF32Waves, (core.tok_end + kTile - 1) / kTile - core.span_skip);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = r0 + 16 * rt + n;
+    const bool valid = row < total_rows;
+    const int rc = valid ? row : r_last;
+    core.limit[rt] = valid ? cached + rc / G + 1 : 0;
+    core.wlo[rt] = window_start(a.span, cached + rc / G);
+    const float* qrow =
+        (const float*)a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR;
+#pragma unroll
+    for (int c = 0; c < Core::NC; ++c) {
+      core.qv[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!PAD || 16 * c + 4 * g < DR)
+        core.qv[rt][c] = *reinterpret_cast<const f32x4*>(qrow + 16 * c + 4 * g);
+    }
+  }
+  core.init_acc();
+  core.run_single(ntiles);
+
+  f32x4* park = reinterpret_cast<f32x4*>(smem + Lds::park);
+  float* park_m = reinterpret_cast<float*>(smem + Lds::park_m);
+  float* park_l = reinterpret_cast<float*>(smem + Lds::park_l);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int x = 0; x < NX; ++x) park[((w * RT + rt) * NX + x) * kWave + lane] = core.o[rt][x];
+    park_m[(w * RT + rt) * kWave + lane] = core.m_run[rt];
+    park_l[(w * RT + rt) * kWave + lane] = core.l_total(rt);
+  }
+  __syncthreads();
+  for (int t = w; t < RT * NX; t += kF32Waves) {
+    const int rt = t / NX, x = t % NX;
+    const int row = r0 + 16 * rt + n;
+    float M = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kF32Waves; ++v) M = fmaxf(M, park_m[(v * RT + rt) * kWave + lane]);
+    float den = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < kF32Waves; ++v) {
+      const float mv = park_m[(v * RT + rt) * kWave + lane];
+      const float sc = mv == kNegInf ? 0.f : exp2f(mv - M);
+      den += sc * park_l[(v * RT + rt) * kWave + lane];
+      // tile x as the 16 dims from 16 x (a lane parked its 4 dims from f32_dim0)
+      acc += sc * park[((v * RT + rt) * NX + (x & ~3) + g) * kWave + 16 * (x & 3) + n];
+    }
+    if (row >= total_rows) continue;
+    const float inv = den > 0.f ? 1.f / den : 0.f;
+    const int64_t r = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
+    const int d0 = 16 * x + 4 * g;
+    if (!PAD || d0 < DR) store_out4<F32>(a.out, r * DR + d0, acc * inv);
+  }
+}
+
+template <int D, bool PAD>
+int launch_f32(const SpanPrefill& a, hipStream_t s) {
+  // two row tiles halve the K/V reads per product, and the workgroups (the plain fp32
+  // prefill's rule and figures: prefill.hip)
+  const int64_t rows = (int64_t)a.total_q * a.G;
+  const int rt = rows * a.Hkv >= 20480 && rows >= (int64_t)48 * a.S ? 2 : 1;
+  const int64_t units = (rows + 16 * rt - 1) / (16 * rt) + a.S;
+  if (units * a.Hkv >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)(units * a.Hkv)), block(kF32Waves * kWave);
+  if (rt == 2)
+    hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD, 2>), grid, block, (SpanF32Lds<D, 2>::bytes),
+                       s, a);
+  else
+    hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD, 1>), grid, block, (SpanF32Lds<D, 1>::bytes),
+                       s, a);
+  return FE_LAUNCH_STATUS();
+}
+
+int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v_pool,
+                     int num_blocks, const int32_t* tables, int table_stride, const int32_t* q_off,
+                     const int32_t* ctx, int num_seqs, int total_q, int hq, int hkv, int d, int bs,
+                     float scale, int window, int sinks, fe_stream_t stream) {
+  FE_CHECK_ARG(num_seqs >= 0 && total_q >= 0 && hq > 0 && hkv > 0 && d > 0 && num_blocks > 0 &&
+               table_stride > 0 && window > 0 && sinks >= 0 && hq % hkv == 0 && scale > 0.f);
+  const int bs_log2 = span_log2(bs);
+  if (bs_log2 < 0 || bs % kTile != 0 || d > 128 || d % 8 != 0) return FE_ERR_UNSUPPORTED;
+  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) ||
+      (int64_t)num_blocks * bs >= ((int64_t)1 << 31) || (int64_t)hkv * d >= ((int64_t)1 << 25) ||
+      (int64_t)total_q * (hq / hkv) >= ((int64_t)1 << 30))
+    return FE_ERR_UNSUPPORTED;
+  if (num_seqs == 0 || total_q == 0) return FE_OK;
+  FE_CHECK_ARG(q && out && k_pool && v_pool && tables && q_off && ctx);
+  const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
+  SpanPrefill a{};
+  a.q = (const f16*)q;
+  a.out = (f16*)out;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.tables = tables;
+  a.q_off = q_off;
+  a.ctx = ctx;
+  a.W = table_stride;
+  a.S = num_seqs;
+  a.total_q = total_q;
+  a.Hq = hq;
+  a.Hkv = hkv;
+  a.G = hq / hkv;
+  a.BS = bs;
+  a.bs_log2 = bs_log2;
+  a.NB = num_blocks;
+  a.KS = 1;
+  a.dr = d;
+  a.scale_log2 = scale * kLog2e;
+  a.span = Span{window, sinks};
+  const hipStream_t s = (hipStream_t)stream;
+  if (d == 64) return launch_f32<64, false>(a, s);
+  if (d == 128) return launch_f32<128, false>(a, s);
+  return d < 64 ? launch_f32<64, true>(a, s) : launch_f32<128, true>(a, s);
+}
+
+}  // namespace
+
+extern "C" size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int num_q_heads,
+                                                 int kv_heads, int head_dim) {
+  if (num_seqs < 0 || total_q < 0 || num_q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
+      num_q_heads % kv_heads)
+    return 0;
+  return span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim).bytes;
+}
+
+#define FE_WINDOW_PREFILL(SUFFIX, E)                                                              \
+  extern "C" int fe_prefill_paged_window##SUFFIX(                                                 \
+      const void* q, void* out, const void* k_pool, const void* v_pool, int num_blocks,           \
+      const int32_t* block_tables, int table_stride, const int32_t* q_offsets,                    \
+      const int32_t* context_lens, int num_seqs, int total_q, int num_q_heads, int kv_heads,      \
+      int head_dim, int block_size, float scale, int window, int sinks, void* workspace,          \
+      size_t workspace_bytes, fe_stream_t stream) {                                               \
+    return span_prefill<E, false>(q, out, k_pool, nullptr, v_pool, nullptr, num_blocks,           \
+                                  block_tables, table_stride, q_offsets, context_lens, num_seqs,  \
+                                  total_q, num_q_heads, kv_heads, head_dim, block_size, scale,    \
+                                  window, sinks, workspace, workspace_bytes, stream);             \
+  }
+FE_WINDOW_PREFILL(, Fp16)
+FE_WINDOW_PREFILL(_bf16, Bf16)
+
+extern "C" int fe_prefill_paged_window_f32(const void* q, void* out, const void* k_pool,
+                                           const void* v_pool, int num_blocks,
+                                           const int32_t* block_tables, int table_stride,
+                                           const int32_t* q_offsets, const int32_t* context_lens,
+                                           int num_seqs, int total_q, int num_q_heads,
+                                           int kv_heads, int head_dim, int block_size, float scale,
+                                           int window, int sinks, void*, size_t,
+                                           fe_stream_t stream) {
+  return span_prefill_f32(q, out, k_pool, v_pool, num_blocks, block_tables, table_stride,
+                          q_offsets, context_lens, num_seqs, total_q, num_q_heads, kv_heads,
+                          head_dim, block_size, scale, window, sinks, stream);
+}

@@ -662,16 +662,23 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                   block_tables: torch.Tensor, q_offsets: torch.Tensor,
                   context_lens: torch.Tensor, max_q_len: int, *, scale: float | None = None,
                   out: torch.Tensor | None = None,
-                  plan: PrefillPlan | None = None) -> torch.Tensor:
+                  plan: PrefillPlan | None = None, window: int | None = None, sinks: int = 0,
+                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Ragged causal prefill: q [total_q, Hq, D]; sequence s owns rows
     q_offsets[s]:q_offsets[s+1] at positions context_lens[s]-n_s .. context_lens[s]-1.
     fp16, bf16 or float32 (q, out and the pools alike).  With `plan`
     (prefill_paged_plan on these q_offsets / context_lens and sizes; 16-bit pools)
     the launch reads its work split from it (fe_prefill_paged_planned); same results.
     Tables no wider than the longest context let it choose the fastest kernel
-    (prefill_form): it takes the width for that length."""
+    (prefill_form): it takes the width for that length.
+
+    window: each row attends the last `window` keys up to its position and the first `sinks`
+    of its sequence only (fe_prefill_paged_window).  Pools may be Kv4Pools of q's dtype
+    (fe_prefill_paged_kv4).  Both want block sizes of at least 16, take no plan and have a
+    workspace of their own (fe_span_prefill_workspace_size); the per-device one unless
+    `workspace` (zero-filled uint8) is given."""
     dev = _require_gpu(q, k_pool, v_pool, block_tables, q_offsets, context_lens, out)
-    nb, bs, hkv, d = _check_pool(k_pool, v_pool, KV_DTYPES)
+    nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     if q.ndim != 3 or q.shape[2] != d or q.dtype != k_pool.dtype or not q.is_contiguous():
         raise ValueError("q must be a contiguous [total_q, num_q_heads, head_dim] of the pools' dtype")
     total_q, hq, _ = q.shape
@@ -689,12 +696,28 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    kv4 = isinstance(k_pool, Kv4Pool)
+    if kv4 or window is not None or sinks:
+        window, sinks = _span(window, sinks)
+        if plan is not None:
+            raise ValueError("4-bit pools and windows take no prefill plan")
+        if workspace is None and q.dtype != FP32:
+            workspace = decode_workspace(dev, int(_lib.load().fe_span_prefill_workspace_size(
+                num_seqs, total_q, hq, hkv, d)), kind="span_prefill")
+        pools = _kv4_ptrs(k_pool, v_pool) if kv4 else (k_pool.data_ptr(), v_pool.data_ptr())
+        _lib.call(("fe_prefill_paged_kv4" if kv4 else "fe_prefill_paged_window") + _SFX[q.dtype],
+                  q.data_ptr(), out.data_ptr(), *pools, nb, block_tables.data_ptr(),
+                  block_tables.shape[1], q_offsets.data_ptr(), context_lens.data_ptr(), num_seqs,
+                  total_q, hq, hkv, d, bs, float(scale), window, sinks, _ptr(workspace),
+                  0 if workspace is None else workspace.numel() * workspace.element_size(),
+                  _stream(dev))
+        return out
     need = int(_lib.load().fe_prefill_workspace_size(num_seqs, total_q, hq, hkv, d))
-    ws = decode_workspace(dev, need, kind="prefill")
+    ws = decode_workspace(dev, need, kind="prefill") if workspace is None else workspace
     args = (q.data_ptr(), out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nb,
             block_tables.data_ptr(), block_tables.shape[1], q_offsets.data_ptr(),
             context_lens.data_ptr(), num_seqs, total_q, int(max_q_len), hq, hkv, d, bs,
-            float(scale), ws.data_ptr(), ws.numel())
+            float(scale), ws.data_ptr(), ws.numel() * ws.element_size())
     sfx = _SFX[q.dtype]
     if plan is None:
         _lib.call("fe_prefill_paged" + sfx, *args, _stream(dev))
