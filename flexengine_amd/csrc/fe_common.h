@@ -274,6 +274,9 @@ constexpr int kMaxPieces = 64;
 #define FE_MIN_CHUNK 3
 #endif
 constexpr int kMinChunk = FE_MIN_CHUNK;
+// With few_pieces: a sequence is cut into no more than that many pieces of fewer than
+// kFewChunk quads.
+constexpr int kFewChunk = 8;
 
 // First key of sequence b's suffix (0 without a shared prefix); <= its length.
 __device__ __forceinline__ int suffix_start(const int32_t* tok0, int b, int L) {
@@ -318,7 +321,8 @@ struct WalkAll {
 template <class Walk = WalkAll>
 __device__ __forceinline__ bool find_piece(const int32_t* ctx, const int32_t* tok0, int B,
                                            int max_len, int target, int item, Piece& pc,
-                                           int& total, Walk walk = Walk{}) {
+                                           int& total, Walk walk = Walk{},
+                                           int few_pieces = kMaxPieces) {
   const int lane = lane_id();
   int L0 = 0, s0 = 0;
   if (lane < B) {
@@ -344,7 +348,12 @@ __device__ __forceinline__ bool find_piece(const int32_t* ctx, const int32_t* to
   sum = __builtin_amdgcn_readfirstlane(sum);
   longest = __builtin_amdgcn_readfirstlane(longest);
   int chunk = (sum + target - 1) / target;
-  const int floor_chunk = (longest + kMaxPieces - 1) / kMaxPieces;
+  int floor_chunk = (longest + kMaxPieces - 1) / kMaxPieces;
+  if (few_pieces < kMaxPieces) {
+    const int few = (longest + few_pieces - 1) / few_pieces;
+    const int cap = few < kFewChunk ? few : kFewChunk;
+    floor_chunk = floor_chunk > cap ? floor_chunk : cap;
+  }
   chunk = chunk > floor_chunk ? chunk : floor_chunk;
   chunk = chunk > kMinChunk ? chunk : kMinChunk;
 

@@ -37,6 +37,15 @@ constexpr size_t kTicketBytes = kMaxTickets * sizeof(int);
 constexpr int kMaxContext = 262144;  // kMaxPieces pieces of 64 quads
 // Working workgroups in all that the default split aims at
 constexpr int kDefaultWorkgroups = 512;
+// A row of few keys is cut into at most this many short pieces: joining one costs about a
+// quarter of what computing a quad does.  One row of 16384 tokens in 4 bits (12/2 heads of 128)
+// with 64 / 32 / 16: 14.8 / 12.6 / 14.1 us; of 100000, whose pieces are long, 24.6.
+constexpr int kFewPieces = 32;
+// Tiles of a wave from which a 4-bit walk takes them two at a time, which has the matrix
+// instructions with V take 32 keys and one round of the softmax serve both, but computes an odd
+// last tile twice over: 37 rows of 2048-16384 tokens (32/8 heads of 128) one / two at a time
+// 70.3 / 67.4 us (the loads alone 63), 64 rows of 128-4096 (12/2 heads) 11.5 / 12.6.
+constexpr int kPairTiles = 16;
 
 struct SpanArgs {
   const f16* q;
@@ -208,6 +217,7 @@ struct Rows4 {
   __device__ __forceinline__ void load_half(const uint8_t* codes, const uint8_t* scales, int row,
                                             int rows, Half& t) const {
     const int cb = dr / 2, sb = dr / kQ4Block;
+    rows = rows > 0 ? rows : 0;
     const __amdgpu_buffer_rsrc_t cr = uniform_rsrc(codes + (int64_t)row * cb, rows * cb);
     const __amdgpu_buffer_rsrc_t sr = uniform_rsrc(scales + (int64_t)row * sb, rows * sb);
     const int n = lane_id() & 15;
@@ -320,9 +330,21 @@ struct Rows4 {
 
 // ---- the walk of one wave ----------------------------------------------------------------
 
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// Maximum over the four lanes of a column (n, n + 16, n + 32, n + 48): permlane swaps, both
+// halves of which are used, in the place of two LDS round trips
+__device__ __forceinline__ float max_of_column(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// A wave's tiles, NT of them (1 or 2) at a time
 template <int D, class E, class Rows>
 struct SpanCore {
   using C = TileCfg<D>;
+  using Tile = typename Rows::Tile;
   Rows rows;
   int L;          // context length
   int sinks, ws;  // keys below sinks and from ws on are seen
@@ -337,40 +359,58 @@ struct SpanCore {
   float m_run, l_run;
   f32x4 o[C::NX];
 
+  // position of tile k's first key (L past the list: no key of it is seen)
   __device__ __forceinline__ int tile_tok(int k) const {
-    return __builtin_amdgcn_readlane(tok_vec, k & (kWave - 1));
+    const int t = __builtin_amdgcn_readlane(tok_vec, k & (kWave - 1));
+    return k < ntiles ? t : L;
   }
-  __device__ __forceinline__ void load(int k, typename Rows::Tile& t) const {
-    const int left = L - tile_tok(k);
-    // no keys past the list's end; keys past the context read as zeros
-    rows.load(__builtin_amdgcn_readlane(row_vec, k & (kWave - 1)),
-              k < ntiles ? (left < kTile ? left : kTile) : 0, t);
+  template <int NT>
+  __device__ __forceinline__ void load(int k0, Tile (&t)[NT]) const {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      // keys past the context read as zeros, tiles past the list are not read
+      const int left = L - tile_tok(k0 + i);
+      rows.load(__builtin_amdgcn_readlane(row_vec, (k0 + i) & (kWave - 1)),
+                left < kTile ? left : kTile, t[i]);
+    }
   }
   __device__ __forceinline__ bool sees(int tok) const {
     return tok < L && (tok < sinks || tok >= ws);
   }
-  __device__ __forceinline__ void compute(int k, typename Rows::Tile& t) {
+  template <int NT>
+  __device__ __forceinline__ void compute(int k0, Tile (&t)[NT]) {
     const int lane = lane_id();
     const int g = lane >> 4;
     const int n = lane & 15;
-    const int t0 = tile_tok(k);
-    if (k == new_tile) rows.put_new(fresh, new_row, t);
-    f32x4 sacc = {0.f, 0.f, 0.f, 0.f};
+    if (new_tile >= k0 && new_tile < k0 + NT)
 #pragma unroll
-    for (int s = 0; s < C::NK; ++s) sacc = mma32<E>(rows.key(t, s), qv[s], sacc);
-    // whole tiles need no mask
-    const bool whole = t0 + kTile <= L && (t0 >= ws || t0 + kTile <= sinks);
-    if (!whole) rows.hide(t, [&](int r) { return sees(t0 + r); });
-    compiler_fence();
-    rows.stage_v(t, stage);
-    compiler_fence();
-    float sv[4];
+      for (int i = 0; i < NT; ++i)
+        if (k0 + i == new_tile) rows.put_new(fresh, new_row, t[i]);
+    float sv[NT][4];
+    f32x4 sacc[NT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      sv[i] = whole || sees(t0 + 4 * g + i) ? sacc[i] * scale_log2 : kNegInf;
-    float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-    mx = fmaxf(mx, shfl_xor_f(mx, 16));
-    mx = fmaxf(mx, shfl_xor_f(mx, 32));
+    for (int i = 0; i < NT; ++i) sacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < C::NK; ++s)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sacc[i] = mma32<E>(rows.key(t[i], s), qv[s], sacc[i]);
+    float mx = kNegInf;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int t0 = tile_tok(k0 + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sv[i][j] = sacc[i][j] * scale_log2;
+      // whole tiles need no mask
+      if (!(t0 + kTile <= L && (t0 >= ws || t0 + kTile <= sinks))) {
+        rows.hide(t[i], [&](int r) { return sees(t0 + r); });
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!sees(t0 + 4 * g + j)) sv[i][j] = kNegInf;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = vmax(mx, sv[i][j]);
+    }
+    mx = max_of_column(mx);
     if (__ballot(mx > m_run + kRescaleSlack)) {  // wave-uniform
       const float m_new = fmaxf(m_run, mx);
       const float alpha = m_new == kNegInf ? 1.f : exp2_fast(m_run - m_new);
@@ -380,37 +420,64 @@ struct SpanCore {
       m_run = m_new;
     }
     const float m_use = m_run == kNegInf ? 0.f : m_run;
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = exp2_fast(sv[i] - m_use);
-    l_run += (p[0] + p[1]) + (p[2] + p[3]);
     // probabilities in 16 bits for the matrix instruction (at most 2^kRescaleSlack)
-    const f16x4 pb = to16x4<E>(p[0], p[1], p[2], p[3]);
+    f16x4 pb[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = exp2_fast(sv[i][j] - m_use);
+      l_run += (p[0] + p[1]) + (p[2] + p[3]);
+      pb[i] = to16x4<E>(p[0], p[1], p[2], p[3]);
+    }
     const unsigned char* vb = stage + (4 * g + (n >> 2)) * C::ROWB + (n & 3) * 8;
+    auto vfrag = [&](const unsigned char* at) __attribute__((always_inline)) {
+      return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s16x4*)at));
+    };
+    compiler_fence();
+#pragma unroll
+    for (int i = 0; i < NT; ++i) rows.stage_v(t[i], stage + i * C::STAGE);
+    compiler_fence();
 #pragma unroll
     for (int x = 0; x < C::NX; ++x) {
-      const s16x4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(vb + 32 * x));
-      o[x] = mma16<E>(__builtin_bit_cast(f16x4, raw), pb, o[x]);
+      const f16x4 a = vfrag(vb + 32 * x);
+      if constexpr (NT == 2) {
+        const f16x4 b = vfrag(vb + C::STAGE + 32 * x);
+        o[x] = mma32<E>(f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]},
+                        f16x8{pb[0][0], pb[0][1], pb[0][2], pb[0][3], pb[1][0], pb[1][1], pb[1][2],
+                              pb[1][3]},
+                        o[x]);
+      } else {
+        o[x] = mma16<E>(a, pb[0], o[x]);
+      }
     }
     compiler_fence();
   }
-  // two tiles in registers: while tile k is computed, the loads of tile k + 1 are in flight
+  // two sets of tiles in registers: while one is computed, the loads of the next are in flight
+  template <int NT>
+  __device__ __forceinline__ void run_by() {
+    Tile ta[NT], tb[NT];
+    load(0, ta);
+    for (int k = 0;; k += 2 * NT) {
+      load(k + NT, tb);
+      if (k >= ntiles) break;
+      compute(k, ta);
+      load(k + 2 * NT, ta);
+      if (k + NT >= ntiles) break;
+      compute(k + NT, tb);
+    }
+  }
+  template <int MAX>
   __device__ __forceinline__ void run() {
     m_run = kNegInf;
     l_run = 0.f;
 #pragma unroll
     for (int x = 0; x < C::NX; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-    typename Rows::Tile ta, tb;
-    load(0, ta);
-    for (int k = 0;; k += 2) {
-      load(k + 1, tb);
-      if (k >= ntiles) break;
-      compute(k, ta);
-      load(k + 2, ta);
-      if (k + 1 >= ntiles) break;
-      compute(k + 1, tb);
+    if constexpr (MAX == 2) {
+      if (ntiles >= kPairTiles) return run_by<2>();
     }
+    run_by<1>();
   }
   __device__ __forceinline__ float l_total() const {
     float l = l_run + shfl_xor_f(l_run, 16);
@@ -420,7 +487,9 @@ struct SpanCore {
 
 // ---- the join of a row's pieces ------------------------------------------------------------
 
-constexpr int kMergeBatch = 16;  // pieces read in one round trip
+// Pieces read in one round trip (16 hold the walk to 2 or 3 waves a SIMD instead of 4: 16-bit
+// windows of 1024, 64 rows of 32/8 heads of 128, 65.2 / 61.1 us)
+constexpr int kMergeBatch = 8;
 
 // out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M) over the ns pieces from slot `first` on;
 // a thread takes 4 dims of a query head
@@ -473,24 +542,32 @@ __device__ __forceinline__ void merge_pieces(const SpanArgs& a, int b, int h, in
   }
 }
 
-// LDS: the waves' V tiles, their states (o, m, l) for the combine, a flag
-template <int D>
+// Tiles that a wave computes at a time, at most
+// (16-bit tiles two at a time: 61.1 -> 65.1 us)
+template <bool Q4>
+constexpr int kTilesAtOnce = Q4 ? 2 : 1;
+
+// LDS: the waves' V tiles, and in their place after the walk the waves' states (o, m, l) for
+// the combine; a flag
+template <int D, int NT>
 struct SpanLds {
-  static constexpr size_t stage = 0;
-  static constexpr size_t park = stage + (size_t)kWaves * TileCfg<D>::STAGE;
-  static constexpr size_t park_m = park + (size_t)kWaves * TileCfg<D>::NX * kWave * 16;
+  static constexpr size_t per_wave = (NT > 1 ? 2 : 1) * TileCfg<D>::STAGE;
+  static constexpr size_t park_m = (size_t)kWaves * TileCfg<D>::NX * kWave * 16;
   static constexpr size_t park_l = park_m + (size_t)kWaves * kWave * sizeof(float);
-  static constexpr size_t flag = park_l + (size_t)kWaves * kWave * sizeof(float);
+  static constexpr size_t parked = park_l + (size_t)kWaves * kWave * sizeof(float);
+  static constexpr size_t flag = parked > kWaves * per_wave ? parked : kWaves * per_wave;
   static constexpr size_t bytes = flag + sizeof(int);
 };
 
 template <int D, class E, bool Q4, bool PAD>
 __global__ __launch_bounds__(kThreads)
-// (D = 256: one wave per SIMD, as the plain decode)
-__attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2, 8)))
+// (D = 256: one wave per SIMD, as the plain decode.  4-bit: four waves a SIMD against the
+// latency of a tile's chain, 74 -> 67 us for the long rows above; the padded form spills there)
+__attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : (Q4 ? (PAD ? 3 : 4) : 2), 8)))
 void span_decode_kernel(const SpanArgs a) {
   using C = TileCfg<D>;
-  using Lds = SpanLds<D>;
+  constexpr int NT = kTilesAtOnce<Q4>;
+  using Lds = SpanLds<D, NT>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int DR = PAD ? a.dr : D;
   const int h = blockIdx.x % a.Hkv;
@@ -507,7 +584,8 @@ void span_decode_kernel(const SpanArgs a) {
   const auto walk = [&](int L) __attribute__((always_inline)) {
     return L - kTile * span_skip(a.span, window_start(a.span, L - 1), kTile);
   };
-  if (!find_piece(a.ctx, nullptr, a.B, a.max_len, a.target, item, pc, total, walk)) {
+  if (!find_piece(a.ctx, nullptr, a.B, a.max_len, a.target, item, pc, total, walk,
+                  kFewPieces)) {
     // past the last piece: zero rows of empty sequences
     const int b = item - total;
     if (b < a.B && seq_len(a.ctx, b, a.max_len) == 0)
@@ -580,7 +658,7 @@ void span_decode_kernel(const SpanArgs a) {
     core.sinks = a.span.sinks;
     core.ws = ws;
     core.scale_log2 = a.scale_log2;
-    core.stage = smem + Lds::stage + w * C::STAGE;
+    core.stage = smem + w * Lds::per_wave;
     core.ntiles = t_first < t_end ? (t_end - t_first + kWaves - 1) / kWaves : 0;
     int blk = 0, tok = 0;
     if (lane < core.ntiles) {
@@ -606,7 +684,7 @@ void span_decode_kernel(const SpanArgs a) {
         core.rows.load_new(a.k_new + new_row, a.v_new + new_row, core.fresh);
       }
     }
-    core.run();
+    core.template run<NT>();
     if (core.new_tile >= 0) {
       // (no page write through a table entry that is not a block)
       const int id = __builtin_amdgcn_readlane(blk, core.new_tile);
@@ -621,7 +699,8 @@ void span_decode_kernel(const SpanArgs a) {
   }
 
   // ---- combine the four waves through LDS: wave w takes output tiles w XW .. +XW ----
-  f32x4* park = reinterpret_cast<f32x4*>(smem + Lds::park);  // [4][NX][64]
+  __syncthreads();  // the V tiles are done with
+  f32x4* park = reinterpret_cast<f32x4*>(smem);  // [4][NX][64]
   float* park_m = reinterpret_cast<float*>(smem + Lds::park_m);
   float* park_l = reinterpret_cast<float*>(smem + Lds::park_l);
   int* flag = reinterpret_cast<int*>(smem + Lds::flag);
@@ -730,7 +809,7 @@ inline SpanWorkspace workspace_of(int batch, int hq, int d, int target) {
 template <int D, class E, bool Q4, bool PAD>
 int launch(const SpanArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((span_decode_kernel<D, E, Q4, PAD>), dim3((a.target + 2 * a.B) * a.Hkv),
-                     dim3(kThreads), SpanLds<D>::bytes, s, a);
+                     dim3(kThreads), (SpanLds<D, kTilesAtOnce<Q4>>::bytes), s, a);
   return FE_LAUNCH_STATUS();
 }
 template <class E, bool Q4>
