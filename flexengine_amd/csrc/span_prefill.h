@@ -39,6 +39,13 @@ namespace fe {
 namespace {
 
 constexpr int kSpanKeys = 64;      // keys per staged block
+// Workgroups that run at once (two of four waves on each of 256 CUs)
+constexpr int kSpanSlots = 512;
+// Key splits: units of fewer blocks than kSpanSplitFrom are not split (500 fresh tokens of 12/2
+// heads in two 26.6 us, whole 20.2), and a split has kSpanShare blocks at least (eight chunks of
+// 64 over up to 4000: 4 blocks 61.7 us, 6 44.0, 8 44.0; one of 16: 25.9, 25.8, 28.9).
+constexpr int kSpanSplitFrom = 12;
+constexpr int kSpanShare = 6;
 constexpr int kSpanMaxSplits = 16;
 constexpr int kSpanTickets = 65536;
 constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
@@ -63,20 +70,51 @@ struct SpanPrefill {
   float* part_lse;  // [KS][total_q * Hq]
   int* tickets;     // [units bound][Hkv], zero between calls
   int W, S, total_q, Hq, Hkv, G, BS, bs_log2, NB, KS;
-  int split_blocks;  // key blocks a split has at least
   int dr;            // the real head_dim (PAD: below D)
   float scale_log2;
   Span span;
+};
+
+// The 16-key tiles that a run of query rows walks: those of the sinks, then those from the one
+// that holds the first row's window start to the last row's position
+struct SpanWalk {
+  int head, skip;  // tiles head, head + 1, ... of the walk are `skip` tiles further on
+  int key_end, ws, sinks;
+  __device__ __forceinline__ void init(const Span& sp, int first_pos, int last_pos) {
+    key_end = last_pos + 1;
+    sinks = sp.sinks;
+    ws = window_start(sp, first_pos);
+    head = (int)(((unsigned)sp.sinks + kTile - 1) / kTile);
+    skip = span_skip(sp, ws, kTile);
+  }
+  // 64-key blocks of four tiles
+  __device__ __forceinline__ int blocks() const {
+    return ((key_end + kTile - 1) / kTile - skip + 3) / 4;
+  }
+  // first key of tile t (past the last one: keys past key_end)
+  __device__ __forceinline__ int key(int t) const { return (t < head ? t : t + skip) * kTile; }
+  __device__ __forceinline__ bool sees(int k) const {
+    return k < key_end && (k < sinks || k >= ws);
+  }
 };
 
 // A unit of work: rows r0 .. r0 + ROWS - 1 (fewer at the end) of sequence s
 struct SpanUnit {
   int s, block, n, q0, ctx;
 };
+// All units of one KV head: how many, and about how many key blocks they walk (each sequence's
+// mean of its first and last unit's)
+struct SpanWork {
+  int units, blocks;
+};
+// Finds unit `item`, and with key splits counts the work.
 template <int ROWS>
-__device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUnit& u) {
+__device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUnit& u,
+                                          SpanWork& work) {
   const int lane = lane_id();
   int carry = 0;
+  bool found = false;
+  work = SpanWork{0, 0};
   for (int base = 0; base < a.S; base += kWave) {
     const int s = base + lane < a.S ? base + lane : a.S - 1;
     const int e0 = a.q_off[s], e1 = a.q_off[s + 1], cx = clamp_len(a.ctx[s]);
@@ -84,6 +122,14 @@ __device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUn
     const int q0 = min(max(e0, 0), a.total_q);
     const int n = base + lane < a.S ? max(min(e1, a.total_q) - q0, 0) : 0;
     const int nb = (int)(((int64_t)n * a.G + ROWS - 1) / ROWS);
+    if (a.KS > 1) {
+      const int ctx = min(cx, a.W * a.BS), cached = ctx >= n ? ctx - n : 0;
+      const int step = min(n, (ROWS + a.G - 1) / a.G);
+      SpanWalk f, l;
+      f.init(a.span, cached, cached + step - 1);
+      l.init(a.span, cached + n - step, cached + n - 1);
+      work.blocks += wave_sum_i(n > 0 ? (f.blocks() + l.blocks()) * nb / 2 : 0);
+    }
     const int incl = wave_scan_incl_i(nb) + carry;
     const unsigned long long hit = __ballot(item >= incl - nb && item < incl);
     if (hit) {
@@ -93,23 +139,29 @@ __device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUn
       u.n = readlane_i(n, src);
       u.q0 = readlane_i(q0, src);
       u.ctx = readlane_i(cx, src);
-      return true;
+      found = true;
+      if (a.KS == 1) return true;
     }
     carry = readlane_i(incl, kWave - 1);
   }
-  return false;
+  work.units = carry;
+  return found;
 }
 
-template <int D>
+template <int D, bool Q4>
 struct SpanCfg {
   static constexpr int ROWB = D * 2;                // LDS bytes per staged key row
   static constexpr int MAT = kSpanKeys * ROWB;
   static constexpr int CPR = D / 8;                 // 16-byte chunks per row
   static constexpr int RPI = kWave / CPR;           // rows per DMA instruction
-  // chunk swizzles of row r (K: 32 rows read one chunk each; V: 4 rows x 64 bytes)
+  // Chunk swizzles of row r.  Reads: K 32 rows, one chunk each; V 4 rows x 64 bytes, so V's
+  // quads of chunks move together.  Writes of 4-bit rows: 4 (D = 64: 8) rows, one chunk of each
+  // quad, so V's chunks move within their quads too (4095 tokens of 32/8 heads 179 -> 173 us;
+  // the DMA of 16-bit rows is slower for it, 165 -> 169 us under a window of 1024).
   static __device__ __forceinline__ int swz_k(int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); }
   static __device__ __forceinline__ int swz_v(int r) {
-    return D >= 128 ? ((r & 3) << 2) : (((r >> 1) & 1) << 2);
+    const int quad = D >= 128 ? (r & 3) : ((r >> 1) & 1);
+    return quad << 2 | (Q4 ? (D >= 128 ? r & 3 : (r >> 1) & 3) : 0);
   }
 };
 
@@ -140,12 +192,12 @@ struct SpanRows {
   f32x16 o[D / 32];
 };
 
-// One staged block whose first key is t0.  mask: some row does not see all of it.
-template <int D, class E>
-__device__ __forceinline__ void span_block(int t0, const unsigned char* kst, const unsigned char* vst,
-                                           bool mask, int sinks, float scale_log2, bool follow,
-                                           SpanRows<D>& r) {
-  using C = SpanCfg<D>;
+// One staged block, tiles t .. t + 3 of the walk.  mask: some row does not see all of it.
+template <int D, class E, bool Q4>
+__device__ __forceinline__ void span_block(const SpanWalk& wk, int t, const unsigned char* kst,
+                                           const unsigned char* vst, bool mask, float scale_log2,
+                                           bool follow, SpanRows<D>& r) {
+  using C = SpanCfg<D, Q4>;
   constexpr int NC = D / 16, NT = D / 32;
   const int lane = lane_id();
   const int hf = lane >> 5;
@@ -188,16 +240,20 @@ __device__ __forceinline__ void span_block(int t0, const unsigned char* kst, con
     for (int x = 0; x < NT; ++x) vf[s][x] = vfrag(s, x);
 
   if (mask) {  // wave-uniform
-    int past = r.pos - t0 - 4 * hf, before = r.lo - t0 - 4 * hf, sink = sinks - t0 - 4 * hf;
-    // (defined here as far as the compiler knows: otherwise it hoists the comparisons out of
-    // the branch)
-    asm volatile("" : "+v"(past), "+v"(before), "+v"(sink));
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = 32 * kt + 8 * (i / 4) + i % 4;
-        if (key > past || (key < before && key >= sink)) st[kt][i] = kNegInf;
+      for (int half = 0; half < 2; ++half) {
+        const int k0 = wk.key(t + 2 * kt + half) + 4 * hf;  // the lane's first key of the tile
+        int past = r.pos - k0, before = r.lo - k0, sink = wk.sinks - k0;
+        // (defined here as far as the compiler knows: otherwise it hoists the comparisons out
+        // of the branch)
+        asm volatile("" : "+v"(past), "+v"(before), "+v"(sink));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = 8 * (i / 4) + i % 4;
+          if (key > past || (key < before && key >= sink)) st[kt][8 * half + i] = kNegInf;
+        }
       }
   }
   float mx = st[0][0];
@@ -239,24 +295,10 @@ __device__ __forceinline__ void span_block(int t0, const unsigned char* kst, con
     }
 }
 
-// What a unit reads: the blocks of its walk, and which keys any of its rows sees
-struct SpanWalk {
-  int head, skip;        // blocks head, head + 1, ... of the walk are `skip` blocks further on
-  int key_end, ws, sinks;
-  __device__ __forceinline__ int block(int j) const { return j < head ? j : j + skip; }
-  __device__ __forceinline__ bool sees(int key) const {
-    return key < key_end && (key < sinks || key >= ws);
-  }
-  // every key of t0 .. t0 + n - 1
-  __device__ __forceinline__ bool sees_all(int t0, int n) const {
-    return t0 + n <= key_end && (t0 >= ws || t0 + n <= sinks);
-  }
-};
-
 // 16-bit pools: wave w brings keys RUN w .. +RUN of a block by LDS DMA
 template <int D, bool PAD, int NW>
 struct Stage16 {
-  using C = SpanCfg<D>;
+  using C = SpanCfg<D, false>;
   static constexpr int RUN = kSpanKeys / NW;
   static constexpr int NI = RUN / C::RPI;
   static_assert(RUN <= 16 && NI >= 1, "a run lies in one page");
@@ -264,10 +306,15 @@ struct Stage16 {
   int idv;              // lane j: pool block of this wave's run of walk block id_base + j
   uint32_t vk[NI], vv[NI];  // lane offsets of the DMA, the swizzles applied
 
+  // first key of this wave's run of walk block j
+  __device__ __forceinline__ int run_key(const SpanWalk& wk, int j) const {
+    return wk.key(4 * j + RUN * w / kTile) + (RUN * w) % kTile;
+  }
+
   __device__ __forceinline__ void load_ids(const SpanPrefill& a, const SpanWalk& wk,
                                            const int32_t* trow, int base) {
     id_base = base;
-    int page = (wk.block(base + lane_id()) * kSpanKeys + RUN * w) >> a.bs_log2;
+    int page = run_key(wk, base + lane_id()) >> a.bs_log2;
     page = page < a.W ? page : a.W - 1;
     idv = trow[page];
   }
@@ -293,7 +340,7 @@ struct Stage16 {
       load_ids(a, wk, trow, j);
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     }
-    const int t0 = wk.block(j) * kSpanKeys + RUN * w;
+    const int t0 = run_key(wk, j);
     const int id = clamp_block(__builtin_amdgcn_readlane(idv, j - id_base), a.NB);
     const int rs = a.Hkv * a.dr * 2;
     int nv = wk.key_end - t0;
@@ -319,7 +366,7 @@ struct Stage16 {
 // 4-bit pools: a thread's chunks of a block, loaded into registers and converted into LDS
 template <int D, class E, bool PAD, int NW>
 struct Stage4 {
-  using C = SpanCfg<D>;
+  using C = SpanCfg<D, true>;
   static constexpr int T = NW * kWave;
   static constexpr int BPR = D / kQ4Block;                 // chunks (32 dims) per row
   static constexpr int CHUNKS = 2 * kSpanKeys * BPR;       // of a block: K's, then V's
@@ -330,27 +377,28 @@ struct Stage4 {
 
   static __device__ __forceinline__ int chunk(int i) { return threadIdx.x + i * T; }
   static __device__ __forceinline__ int key_of(int i) { return chunk(i) / BPR % kSpanKeys; }
+  // position of the key of chunk i of walk block j
+  static __device__ __forceinline__ int key_at(const SpanWalk& wk, int j, int i) {
+    return wk.key(4 * j + key_of(i) / kTile) + key_of(i) % kTile;
+  }
   __device__ __forceinline__ void load_ids(const SpanPrefill& a, const SpanWalk& wk,
                                            const int32_t* trow, int j) {
-    const int t0 = wk.block(j) * kSpanKeys;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      int page = (t0 + key_of(i)) >> a.bs_log2;
+      int page = key_at(wk, j, i) >> a.bs_log2;
       page = page < a.W ? page : a.W - 1;
       id[i] = trow[page];
     }
   }
   __device__ __forceinline__ void load(const SpanPrefill& a, const SpanWalk& wk, int h, int j) {
-    const int t0 = wk.block(j) * kSpanKeys;
     const int cb = a.dr / 2, sb = a.dr / kQ4Block;
-    const bool all = wk.sees_all(t0, kSpanKeys);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int c = chunk(i), key = t0 + key_of(i), blk = c % BPR;
+      const int c = chunk(i), key = key_at(wk, j, i), blk = c % BPR;
       const bool is_v = c >= kSpanKeys * BPR;
       codes[i] = span_u32x4{0, 0, 0, 0};
       scale[i] = kQ4ScaleLow;
-      if (c < CHUNKS && (!PAD || blk < sb) && (all || wk.sees(key))) {
+      if (c < CHUNKS && (!PAD || blk < sb) && wk.sees(key)) {
         const int64_t row =
             ((int64_t)clamp_block(id[i], a.NB) * a.Hkv + h) * a.BS + (key & (a.BS - 1));
         const uint8_t* cp = (const uint8_t*)(is_v ? a.v_pool : a.k_pool);
@@ -380,7 +428,7 @@ template <int D, class E, bool Q4, bool PAD, int NW>
 __global__ __launch_bounds__(NW* kWave)
 __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2, D > 128 ? 1 : 2)))
 void span_prefill_kernel(const SpanPrefill a) {
-  using C = SpanCfg<D>;
+  using C = SpanCfg<D, Q4>;
   constexpr int ROWS = 32 * NW;
   // one LDS object per stage and matrix: the compiler's wait for an LDS DMA before an LDS read
   // is then limited to reads of the object it fills
@@ -389,15 +437,15 @@ void span_prefill_kernel(const SpanPrefill a) {
   __shared__ __align__(16) unsigned char k1[C::MAT];
   __shared__ __align__(16) unsigned char v1[C::MAT];
   __shared__ int last;
-  // workgroup i: (KV head, key split) pair i % (Hkv KS), the later units, which see more keys,
-  // first
-  const int pairs = a.Hkv * a.KS;
-  const int items = (int)gridDim.x / pairs;
-  const int item = items - 1 - (int)blockIdx.x / pairs;
-  const int h = (int)blockIdx.x % pairs % a.Hkv;
-  const int ks = (int)blockIdx.x % pairs / a.Hkv;
+  // Workgroups in the order of their split, within it the later units, which see more keys,
+  // first: those without work (a unit has as many splits as its keys are worth) come last
+  const int items = (int)gridDim.x / (a.Hkv * a.KS);
+  const int h = (int)blockIdx.x % a.Hkv;
+  const int ks = (int)blockIdx.x / a.Hkv / items;
+  const int item = items - 1 - (int)blockIdx.x / a.Hkv % items;
   SpanUnit u;
-  if (!find_unit<ROWS>(a, item, u)) return;
+  SpanWork work;
+  if (!find_unit<ROWS>(a, item, u, work)) return;
   const int G = a.G;
   const int DR = PAD ? a.dr : D;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -411,15 +459,19 @@ void span_prefill_kernel(const SpanPrefill a) {
   const int r_last = min(r0 + ROWS, total_rows) - 1;
 
   SpanWalk wk;
-  wk.key_end = cached + r_last / G + 1;
-  wk.sinks = a.span.sinks;
-  wk.ws = window_start(a.span, cached + r0 / G);
-  wk.head = (int)(((unsigned)wk.sinks + kSpanKeys - 1) / kSpanKeys);
-  wk.skip = span_skip(a.span, wk.ws, kSpanKeys);
-  const int nb = (wk.key_end + kSpanKeys - 1) / kSpanKeys - wk.skip;
-  // splits of this unit: no shorter than split_blocks
-  int splits = nb / a.split_blocks;
-  splits = splits < 1 ? 1 : (splits > a.KS ? a.KS : splits);
+  wk.init(a.span, cached + r0 / G, cached + r_last / G);
+  const int nb = wk.blocks();
+  int splits = 1;
+  if (a.KS > 1 && nb >= kSpanSplitFrom) {
+    // splits of equal shares of the work, so that all of them fit the chip at once: the
+    // units' last ones may be short, at most one more workgroup a unit
+    const int slots = kSpanSlots - work.units * a.Hkv;
+    if (slots > 0) {
+      const int share =
+          max((int)(((int64_t)work.blocks * a.Hkv + slots - 1) / slots), kSpanShare);
+      splits = min((nb + share - 1) / share, a.KS);
+    }
+  }
   if (ks >= splits) return;
   const int j0 = (int)((int64_t)nb * ks / splits), j1 = (int)((int64_t)nb * (ks + 1) / splits);
 
@@ -447,11 +499,11 @@ void span_prefill_kernel(const SpanPrefill a) {
   }
   auto compute = [&](int j, const unsigned char* kst, const unsigned char* vst)
                      __attribute__((always_inline)) {
-    const int t0 = wk.block(j) * kSpanKeys;
-    const bool sink = t0 + kSpanKeys <= wk.sinks;
-    if (!has_rows || t0 > p_last || (t0 + kSpanKeys <= lo_first && t0 >= wk.sinks)) return;
-    const bool mask = t0 + kSpanKeys - 1 > p_first || (t0 < lo_last && !sink);
-    span_block<D, E>(t0, kst, vst, mask, wk.sinks, a.scale_log2, j - j0 < kSpanFollow, r);
+    // first and last key of the block (a block with both sinks and window keys has a gap)
+    const int k0 = wk.key(4 * j), k1 = wk.key(4 * j + 3) + kTile - 1;
+    if (!has_rows || k0 > p_last || (k1 < lo_first && k0 >= wk.sinks)) return;
+    const bool mask = k1 > p_first || (k0 < lo_last && k1 >= wk.sinks);
+    span_block<D, E, Q4>(wk, 4 * j, kst, vst, mask, a.scale_log2, j - j0 < kSpanFollow, r);
   };
 
   if constexpr (Q4) {
@@ -541,45 +593,61 @@ void span_prefill_kernel(const SpanPrefill a) {
   __syncthreads();
   if (!last) return;
   if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // thread -> (row, 4 dims); four splits read in one round trip
-  constexpr int TPR = D / 4;
+  // thread -> (row, 4 dims); four splits of four rows are read in one round trip
+  constexpr int TPR = D / 4, RPP = NW * kWave / TPR;  // threads a row, rows a pass
   const int d4 = (int)(threadIdx.x % TPR) * 4;
-  for (int row = r0 + (int)threadIdx.x / TPR; row <= r_last; row += NW * kWave / TPR) {
-    const int64_t orow = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
-    float M = kNegInf, den = 0.f;
-    f32x4 num = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < splits; s0 += 4) {
-      float lv[4];
-      f32x4 ov[4];
+  for (int row0 = r0 + (int)threadIdx.x / TPR; row0 <= r_last; row0 += 4 * RPP) {
+    int64_t orow[4];
+    float M[4], den[4];
+    f32x4 num[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = s0 + k < splits ? s0 + k : splits - 1;
-        const uint32_t prow = (uint32_t)(s * split_rows + orow);
-        lv[k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                              rl, prow * (uint32_t)sizeof(float), 0, kSpanSc1));
-        ov[k] = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                       ro, (prow * D + d4) * (uint32_t)sizeof(float), 0, kSpanSc1));
-      }
-      float bm = M;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (s0 + k >= splits) lv[k] = kNegInf;
-        bm = fmaxf(bm, lv[k]);
-      }
-      const float alpha = M == kNegInf ? 0.f : exp2f(M - bm);
-      num *= alpha;
-      den *= alpha;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float wt = lv[k] == kNegInf ? 0.f : exp2f(lv[k] - bm);
-        num += wt * ov[k];
-        den += wt;
-      }
-      M = bm;
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(row0 + i * RPP, r_last);
+      orow[i] = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
+      M[i] = kNegInf;
+      den[i] = 0.f;
+      num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (!PAD || d4 < DR)
-      *reinterpret_cast<f16x4*>(a.out + orow * DR + d4) = to16x4<E>(num * (den > 0.f ? 1.f / den : 0.f));
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+      float lv[4][4];
+      f32x4 ov[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int s = s0 + k < splits ? s0 + k : splits - 1;
+          const uint32_t prow = (uint32_t)(s * split_rows + orow[i]);
+          lv[i][k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                   rl, prow * (uint32_t)sizeof(float), 0, kSpanSc1));
+          ov[i][k] = __builtin_bit_cast(
+              f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                         ro, (prow * D + d4) * (uint32_t)sizeof(float), 0, kSpanSc1));
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float bm = M[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (s0 + k >= splits) lv[i][k] = kNegInf;
+          bm = fmaxf(bm, lv[i][k]);
+        }
+        const float alpha = M[i] == kNegInf ? 0.f : exp2f(M[i] - bm);
+        num[i] *= alpha;
+        den[i] *= alpha;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float wt = lv[i][k] == kNegInf ? 0.f : exp2f(lv[i][k] - bm);
+          num[i] += wt * ov[i][k];
+          den[i] += wt;
+        }
+        M[i] = bm;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (row0 + i * RPP <= r_last && (!PAD || d4 < DR))
+        *reinterpret_cast<f16x4*>(a.out + orow[i] * DR + d4) =
+            to16x4<E>(num[i] * (den[i] > 0.f ? 1.f / den[i] : 0.f));
   }
 }
 
@@ -601,16 +669,30 @@ struct SpanShape {
   int ks;
   size_t o, lse, bytes;  // workspace
 };
-inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d) {
+// Eight waves a workgroup halve what a row block converts, but leave one workgroup a CU, whose
+// start and end nothing hides: for long prompts over 4-bit pools that fill the chip either way.
+// Four / eight waves, fp16, 32/8 heads of 128: 1000 fresh tokens 38 / 39 us, 2000 64 / 70, 4095
+// (bf16) 173 / 148, 6000 338 / 325 (under a window of 2000 209 / 215, of 4000 302 / 282), four
+// of 1000 67 / 71; four of 2000 of 12/2 heads 97 / 94.  16-bit rows: 8191 tokens under a window
+// of 1024 165 / 189, 6000 under 4000 289 / 289.
+inline int span_waves(int num_seqs, int total_q, int hq, int hkv, int d, int window, bool q4) {
+  const int64_t wgs = ((int64_t)total_q * (hq / hkv) + 255) / 256 * hkv;
+  return q4 && d == 128 && (window == 0 || window >= 4000) && wgs >= 384 &&
+                 total_q / num_seqs >= 2000
+             ? 8
+             : 4;
+}
+inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d, int window, bool q4) {
   SpanShape p;
   const int64_t rows = (int64_t)total_q * (hq / hkv);
-  p.waves = 4;
+  p.waves = span_waves(num_seqs, total_q, hq, hkv, d, window, q4);
   p.units = (rows + 32 * p.waves - 1) / (32 * p.waves) + num_seqs;
-  // key splits so that about 512 workgroups run, two per CU
+  // key splits of a unit at most: twice the slots over the units, for those with more keys
+  // than the others
   const int64_t wgs = ((rows + 32 * p.waves - 1) / (32 * p.waves)) * hkv;
-  int64_t ks = wgs > 0 ? 512 / wgs : 1;
+  int64_t ks = wgs > 0 ? 2 * kSpanSlots / wgs : 1;
   ks = ks < 1 ? 1 : (ks > kSpanMaxSplits ? kSpanMaxSplits : ks);
-  if (p.units * hkv > kSpanTickets) ks = 1;
+  if (p.waves != 4 || p.units * hkv > kSpanTickets) ks = 1;
   const int64_t part_rows = (int64_t)total_q * hq;
   while (ks > 1 && ks * part_rows * span_dim(d) * (int64_t)sizeof(float) >= ((int64_t)1 << 31)) --ks;
   p.ks = (int)ks;
@@ -623,6 +705,12 @@ inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d) {
 template <int D, class E, bool Q4, bool PAD>
 int span_launch(const SpanPrefill& a, const SpanShape& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.units * a.Hkv * a.KS));
+  if constexpr (D == 128 && Q4 && !PAD) {
+    if (p.waves == 8) {
+      hipLaunchKernelGGL((span_prefill_kernel<D, E, Q4, PAD, 8>), grid, dim3(8 * kWave), 0, s, a);
+      return FE_LAUNCH_STATUS();
+    }
+  }
   hipLaunchKernelGGL((span_prefill_kernel<D, E, Q4, PAD, 4>), grid, dim3(4 * kWave), 0, s, a);
   return FE_LAUNCH_STATUS();
 }
@@ -651,7 +739,7 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   if (Q4) FE_CHECK_ARG(k_scales && v_scales);
   const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
-  const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d);
+  const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d, window, Q4);
   if (p.units * hkv * p.ks >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned(workspace))
     return FE_ERR_WORKSPACE;
@@ -678,7 +766,6 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   a.bs_log2 = bs_log2;
   a.NB = num_blocks;
   a.KS = p.ks;
-  a.split_blocks = 4;
   a.dr = d;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, window > 0 ? sinks : 0};

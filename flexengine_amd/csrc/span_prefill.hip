@@ -34,7 +34,8 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   const int h = blockIdx.x % a.Hkv;
   const int item = (int)gridDim.x / a.Hkv - 1 - (int)blockIdx.x / a.Hkv;
   SpanUnit u;
-  if (!find_unit<ROWS>(a, item, u)) return;
+  SpanWork work;
+  if (!find_unit<ROWS>(a, item, u, work)) return;
   const int G = a.G;
   const int lane = lane_id();
   const int g = lane >> 4;
@@ -192,7 +193,8 @@ extern "C" size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int 
   if (num_seqs < 0 || total_q < 0 || num_q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
       num_q_heads % kv_heads)
     return 0;
-  return span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim).bytes;
+  // (the form of eight waves takes no more)
+  return span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim, 1, false).bytes;
 }
 
 #define FE_WINDOW_PREFILL(SUFFIX, E)                                                              \
