@@ -14,8 +14,10 @@ Two entry forms, matching the reference's plugin surface:
 `cache` is anything with the reference PagedKVCache's attributes: `.k` / `.v`
 pools [layers, NB, BS, Hkv, D], `.tables` (request id -> block list) and
 `.layout.kv_heads`; the reference's own PagedKVCache and
-flexengine_amd.kv_cache.PagedKVCache both qualify.  The scale is 1/sqrt(D), as
-in the reference (paged.py:26).  Errors: ValueError for bad shapes or an
+flexengine_amd.kv_cache.PagedKVCache both qualify, the latter with rows held in
+4 bits too.  The scale is 1/sqrt(D), as in the reference (paged.py:26).  All three
+take window / sinks: a query then sees the last `window` keys up to its position and
+the first `sinks` of its sequence (block sizes of at least 16).  Errors: ValueError for bad shapes or an
 unknown backend, RuntimeError when the HIP library or a GPU is missing --
 there is no silent fallback.
 """
@@ -39,7 +41,8 @@ def _check_query(q: torch.Tensor, positions: torch.Tensor, cache) -> int:
 
 
 def attention_for_request(q: torch.Tensor, cache, layer: int, request_id: str, length: int,
-                          positions: torch.Tensor, backend: str = "hip") -> torch.Tensor:
+                          positions: torch.Tensor, backend: str = "hip",
+                          window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """q [Q, Hq, D] at absolute positions `positions` (the last `Q` of `length`
     tokens); returns [Q, Hq, D] in q's dtype, causal per request."""
     _check_query(q, positions, cache)
@@ -62,9 +65,10 @@ def attention_for_request(q: torch.Tensor, cache, layer: int, request_id: str, l
     table, ctx, offs = buf.split((pages, 1, 2))
     table = table.unsqueeze(0)
     if n == 1:
-        return ops.paged_decode(q, cache.k[layer], cache.v[layer], table, ctx, scale=scale)
+        return ops.paged_decode(q, cache.k[layer], cache.v[layer], table, ctx, scale=scale,
+                                window=window, sinks=sinks)
     return ops.prefill_paged(q.contiguous(), cache.k[layer], cache.v[layer], table, offs, ctx, n,
-                             scale=scale)
+                             scale=scale, window=window, sinks=sinks)
 
 
 def context_lens_from_positions(positions: torch.Tensor, active_mask: torch.Tensor) -> torch.Tensor:
@@ -95,8 +99,8 @@ def decode_step_inputs(block_tables: torch.Tensor, positions: torch.Tensor,
 
 def paged_decode_batch(q: torch.Tensor, cache, layer: int, block_tables: torch.Tensor,
                        positions: torch.Tensor, active_mask: torch.Tensor, *,
-                       k_new: torch.Tensor | None = None,
-                       v_new: torch.Tensor | None = None) -> torch.Tensor:
+                       k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None,
+                       window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """Batched single-token decode: q [B, Hq, D], block_tables [B, W] (int32 or int64),
     positions [B] (query position = length - 1), active_mask [B] -> [B, Hq, D].
 
@@ -110,12 +114,15 @@ def paged_decode_batch(q: torch.Tensor, cache, layer: int, block_tables: torch.T
         raise ValueError("Q heads must be a multiple of KV heads")
     tables, ctx = decode_step_inputs(block_tables, positions, active_mask)
     return ops.paged_decode(q, cache.k[layer], cache.v[layer], tables, ctx,
-                            scale=1.0 / math.sqrt(q.shape[-1]), k_new=k_new, v_new=v_new)
+                            scale=1.0 / math.sqrt(q.shape[-1]), k_new=k_new, v_new=v_new,
+                            window=window, sinks=sinks)
 
 
 def prefill_batch(q: torch.Tensor, cache, layer: int, block_tables: torch.Tensor,
-                  q_offsets: torch.Tensor, context_lens: torch.Tensor, max_q_len: int) -> torch.Tensor:
+                  q_offsets: torch.Tensor, context_lens: torch.Tensor, max_q_len: int, *,
+                  window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """Ragged chunked prefill of several requests in one launch (the per-request
     loop of qwen2.py:117-126 fused): q [total_q, Hq, D]."""
     return ops.prefill_paged(q, cache.k[layer], cache.v[layer], block_tables, q_offsets,
-                             context_lens, max_q_len, scale=1.0 / math.sqrt(q.shape[-1]))
+                             context_lens, max_q_len, scale=1.0 / math.sqrt(q.shape[-1]),
+                             window=window, sinks=sinks)

@@ -35,6 +35,9 @@ The organisation underneath is this package's own:
   allocator.py:26), each with its HIP kernels (the _bf16 / _f32 entry points).
   The default here is float16 on "cuda:0", the dtype and place the decode path
   is built around; callers that want the reference's float32 pass it.
+* With bits=4 the float16 or bfloat16 rows are held in 4 bits (ops.Kv4Pool; 3.76
+  times the tokens in the same memory): written and attended through the same calls,
+  materialize() gives the rows' values back; there are no views of rows (iter_blocks).
 """
 from __future__ import annotations
 
@@ -253,7 +256,8 @@ class _DeviceTables:
 # ---------------------------------------------------------------------------------------
 
 class PagedKVCache:
-    def __init__(self, layout: CacheLayout, device="cuda:0", dtype=torch.float16, fill=None):
+    def __init__(self, layout: CacheLayout, device="cuda:0", dtype=torch.float16, fill=None,
+                 bits: int | None = None):
         if dtype not in (torch.float16, torch.bfloat16, torch.float32):
             raise ValueError(f"KV pools are float16, bfloat16 or float32 on the HIP kernels; "
                              f"got {dtype}")
@@ -262,11 +266,20 @@ class PagedKVCache:
         self.dtype = dtype
         shape = (layout.layers, layout.num_blocks, layout.block_size, layout.kv_heads,
                  layout.head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=self.device)
-        self.v = torch.empty(shape, dtype=dtype, device=self.device)
-        if fill is not None:
-            self.k.fill_(fill)
-            self.v.fill_(fill)
+        if bits not in (None, 4):
+            raise ValueError(f"KV rows are held in their own type or in 4 bits; got bits={bits}")
+        self.bits = bits
+        if bits == 4:
+            if fill:
+                raise ValueError("a 4-bit cache starts with rows of zeros; it takes no other fill")
+            self.k = ops.Kv4Pool.empty(shape, dtype, self.device)
+            self.v = ops.Kv4Pool.empty(shape, dtype, self.device)
+        else:
+            self.k = torch.empty(shape, dtype=dtype, device=self.device)
+            self.v = torch.empty(shape, dtype=dtype, device=self.device)
+            if fill is not None:
+                self.k.fill_(fill)
+                self.v.fill_(fill)
         self._ledger = _Ledger(layout.num_blocks)
         self._pt = _PageTables()
         self._dev = _DeviceTables(self.device) if self.device.type == "cuda" else None
@@ -465,6 +478,8 @@ class PagedKVCache:
     def iter_blocks(self, layer: int, request_id: str, length: int):
         """(first position, K page view, V page view) of every page holding one of the
         request's first `length` rows; views of the pool, nothing copied."""
+        if self.bits == 4:
+            raise ValueError("a 4-bit cache has no rows to view; materialize() copies their values")
         if not 0 < length <= self.available_slots(request_id):
             raise ValueError(f"length {length} is not within the reserved slots of {request_id!r}")
         bs = self.layout.block_size

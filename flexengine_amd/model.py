@@ -30,6 +30,10 @@ for decode-sized batches and on the library GEMM (hipBLASLt via torch) above.
 Default configuration: Qwen2.5-1.5B (28 layers, hidden 1536, 12/2 heads,
 head_dim 128, intermediate 8960, vocab 151936, tied embeddings, q/k/v bias,
 RMS eps 1e-6, theta 1e6).
+
+With sliding_window in the configuration every layer's attention sees the last
+that many tokens and the first attention_sinks; a cache made with bits=4 holds its
+rows in 4 bits.  Either runs the same forwards, without the two plans.
 """
 from __future__ import annotations
 
@@ -54,6 +58,8 @@ class Qwen2Config:
     rope_theta: float = 1000000.0
     rms_norm_eps: float = 1e-6
     tie_word_embeddings: bool = True
+    sliding_window: int | None = None  # keys that a token sees up to itself; None: all
+    attention_sinks: int = 0           # first tokens that it sees beside them
 
     @property
     def parameters(self) -> int:
@@ -116,6 +122,9 @@ class Qwen2Model:
         self.inv_freq = 1.0 / cfg.rope_theta ** (
             torch.arange(0, self.dim, 2, device=self.device, dtype=torch.float32) / self.dim)
         self.scale = 1.0 / math.sqrt(self.dim)
+        ops.check_window(cfg.sliding_window, cfg.attention_sinks)
+        self.span = {} if cfg.sliding_window is None else dict(window=cfg.sliding_window,
+                                                               sinks=cfg.attention_sinks)
 
     # ---- building blocks ----------------------------------------------------------
     # Per layer: fused add + RMSNorm, the q/k/v GEMM, RoPE + split, attention, the o
@@ -137,6 +146,9 @@ class Qwen2Model:
         act = ops.silu_mul(ops.linear(h2, lw.w_gate_up))
         h, _ = ops.rmsnorm(ops.linear(act, lw.w_down), next_norm, self.cfg.rms_norm_eps, residual=x)
         return h
+
+    def _unplanned(self, cache) -> bool:
+        return bool(self.span) or isinstance(cache.k, ops.Kv4Pool)
 
     def _next_norm(self, layer: int) -> torch.Tensor:
         return (self.layer_weights[layer + 1].input_norm if layer + 1 < self.layers
@@ -181,10 +193,10 @@ class Qwen2Model:
         ctx = torch.tensor([c.start + n for c, n in zip(chunks, lengths)], dtype=torch.int32).to(dev)
         max_q = max(lengths)
         # the prefill's work split of this step, shared by every layer (None when
-        # the sizes take the tile kernel)
-        plan = ops.prefill_paged_plan(q_offsets, ctx, len(pos_list),
-                                      self.cfg.num_attention_heads, self.cfg.num_key_value_heads,
-                                      width, bs)
+        # the sizes take the tile kernel, and for windows and 4-bit rows)
+        plan = None if self._unplanned(cache) else ops.prefill_paged_plan(
+            q_offsets, ctx, len(pos_list), self.cfg.num_attention_heads,
+            self.cfg.num_key_value_heads, width, bs)
         ends = torch.tensor([sum(lengths[:j + 1]) - 1 for j in range(len(lengths))],
                             dtype=torch.long).to(dev)
         x = self.embed.index_select(0, ids)
@@ -193,7 +205,7 @@ class Qwen2Model:
             q, k, v = self._qkv(h, lw, positions)
             ops.write_kv_ragged(k, v, cache.k[layer], cache.v[layer], tables, q_offsets, ctx)
             attn = ops.prefill_paged(q, cache.k[layer], cache.v[layer], tables, q_offsets, ctx,
-                                     max_q, scale=self.scale, plan=plan)
+                                     max_q, scale=self.scale, plan=plan, **self.span)
             if layer == self.layers - 1:
                 # past the last layer's attention only the last tokens' rows reach the logits
                 x, attn = x.index_select(0, ends), attn.index_select(0, ends)
@@ -217,7 +229,9 @@ class Qwen2Model:
         # the decode plan (split-K partition and block rows) of this step, shared by
         # every layer: the tables and lengths are the same for all of them
         nb, bs, hkv = cache.k[0].shape[0], cache.k[0].shape[1], cache.k[0].shape[2]
-        plan = ops.paged_decode_plan(tables, ctx, nb, hkv, bs) if bs % 16 == 0 else None
+        plan = None
+        if bs % 16 == 0 and not self._unplanned(cache):
+            plan = ops.paged_decode_plan(tables, ctx, nb, hkv, bs)
         x = self.embed.index_select(0, input_ids)
         h, _ = ops.rmsnorm(x, self.layer_weights[0].input_norm, self.cfg.rms_norm_eps)
         if batch <= ops.SKINNY_MAX_ROWS and self.cfg.hidden_size % 32 == 0:
@@ -226,7 +240,7 @@ class Qwen2Model:
             for layer, lw in enumerate(self.layer_weights):
                 q, k, v = self._qkv(h, lw, positions)
                 attn = ops.paged_decode(q, cache.k[layer], cache.v[layer], tables, ctx,
-                                        scale=self.scale, k_new=k, v_new=v, plan=plan)
+                                        scale=self.scale, k_new=k, v_new=v, plan=plan, **self.span)
                 h = self._after_attention(x, attn, lw, self._next_norm(layer))
             logits = self._logits(h)
         return logits * active.to(logits.dtype)[:, None]
@@ -250,7 +264,7 @@ class Qwen2Model:
             q, k, v = ops.gemm_rope(h, lw.w_qkv, lw.b_qkv, positions, self.inv_freq,
                                     self.nq, self.nkv, self.dim)
             attn = ops.paged_decode(q, cache.k[layer], cache.v[layer], tables, ctx, scale=self.scale,
-                                    k_new=k, v_new=v, plan=plan)
+                                    k_new=k, v_new=v, plan=plan, **self.span)
             o_in = attn.reshape(rows, self.nq * self.dim)
             if fused_norm:
                 r1, h2 = ops.gemm_resid_rmsnorm(o_in, lw.w_o, res, lw.post_norm, eps)

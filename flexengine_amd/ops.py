@@ -69,8 +69,13 @@ class Kv4Pool:
     def ndim(self) -> int:
         return self.codes.ndim
 
+    @functools.cached_property
+    def _layers(self) -> list["Kv4Pool"]:
+        return [Kv4Pool(c, s, self.dtype) for c, s in zip(self.codes.unbind(0), self.scales.unbind(0))]
+
     def __getitem__(self, layer: int) -> "Kv4Pool":
-        return Kv4Pool(self.codes[layer], self.scales[layer], self.dtype)
+        """The pool of one layer (views of this one's tensors)."""
+        return self._layers[layer]
 
 
 def _require_gpu(*tensors: torch.Tensor) -> torch.device:
@@ -123,20 +128,23 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor,
 def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
     if not (isinstance(k_pool, Kv4Pool) and isinstance(v_pool, Kv4Pool)):
         raise ValueError("K and V pools must both be 4-bit pools, or both tensors")
-    if k_pool.ndim != 4 or k_pool.codes.shape != v_pool.codes.shape:
+    kc, ks, vc, vs = k_pool.codes, k_pool.scales, v_pool.codes, v_pool.scales
+    shape = kc.shape
+    if len(shape) != 4 or vc.shape != shape:
         raise ValueError("4-bit pools must both hold one layer of [num_blocks, kv_heads, block_size]")
-    nb, hkv, bs, half = k_pool.codes.shape
+    nb, hkv, bs, half = shape
     if k_pool.dtype not in DTYPES_16 or v_pool.dtype != k_pool.dtype:
         raise ValueError("4-bit pools must hold float16 or bfloat16 rows (both the same)")
-    for p in (k_pool, v_pool):
-        if p.codes.dtype != torch.uint8 or p.scales.dtype != torch.uint8 or half % 16 or \
-                p.scales.shape != (nb, hkv, bs, half // 16):
-            raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
-                             "[..., head_dim / 32] (head_dim a multiple of 32)")
-        if not (p.codes.is_contiguous() and p.scales.is_contiguous()):
-            raise ValueError("K/V pools must be contiguous")
-        if p.scales.device != p.codes.device:
-            raise ValueError("a 4-bit pool's codes and scales must be on one device")
+    scales = (nb, hkv, bs, half // 16)
+    if half % 16 or ks.shape != scales or vs.shape != scales or not (
+            kc.dtype is ks.dtype is vc.dtype is vs.dtype is torch.uint8):
+        raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
+                         "[..., head_dim / 32] (head_dim a multiple of 32)")
+    if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("K/V pools must be contiguous")
+    dev = kc.device
+    if ks.device != dev or vs.device != dev:
+        raise ValueError(f"all tensors must be on {dev}")
     return nb, bs, hkv, 2 * half
 
 
@@ -161,8 +169,9 @@ def _kv4_ptrs(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple:
             v_pool.scales.data_ptr())
 
 
-def _span(window: int | None, sinks: int) -> tuple[int, int]:
-    """(window, sinks) as the library takes them (window 0: none)."""
+def check_window(window: int | None, sinks: int = 0) -> tuple[int, int]:
+    """(window, sinks) as the library takes them (window 0: none); ValueError for a window
+    below 1, negative sinks, or sinks without a window."""
     sinks = operator.index(sinks)
     if window is None:
         if sinks:
@@ -411,7 +420,7 @@ def _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_
             raise ValueError("k_new/v_new heads must be contiguous with equal strides")
         new_stride = k_new.stride(0)
     if out is None:
-        out = torch.empty((batch, hq, d), dtype=dt, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (batch, hq, d) or out.dtype != dt or not out.is_contiguous():
         raise ValueError("out must be a contiguous [batch, num_q_heads, head_dim] of q's dtype")
     if scale is None:
@@ -481,7 +490,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
     kv4 = isinstance(k_pool, Kv4Pool)
     if kv4 or window is not None or sinks:
-        window, sinks = _span(window, sinks)
+        window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no decode plan")
         if workspace is None:
@@ -698,7 +707,7 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         scale = 1.0 / math.sqrt(d)
     kv4 = isinstance(k_pool, Kv4Pool)
     if kv4 or window is not None or sinks:
-        window, sinks = _span(window, sinks)
+        window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no prefill plan")
         if workspace is None and q.dtype != FP32:
