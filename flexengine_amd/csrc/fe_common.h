@@ -178,20 +178,26 @@ __device__ __forceinline__ f32x16 mma32x32(f16x8 a, f16x8 b, f32x16 c) {
 }
 typedef f16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-// c + the sum of 8 elements of type E
+// c + the sum of 2, 4 or 8 elements of type E
 template <class E>
-__device__ __forceinline__ float sum8(f16x8 v, float c) {
+__device__ __forceinline__ float sum2(f16 a, f16 b, float c) {
   const f16 one = __is_same(E, Bf16) ? __builtin_bit_cast(f16, (__bf16)1.f) : (f16)1.f;
   const f16x2_t ones = {one, one};
+  const f16x2_t x = {a, b};
+  if constexpr (__is_same(E, Bf16))
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x),
+                                           __builtin_bit_cast(bf16x2_t, ones), c, false);
+  else
+    return __builtin_amdgcn_fdot2(x, ones, c, false);
+}
+template <class E>
+__device__ __forceinline__ float sum4(f16x4 v, float c) {
+  return sum2<E>(v[2], v[3], sum2<E>(v[0], v[1], c));
+}
+template <class E>
+__device__ __forceinline__ float sum8(f16x8 v, float c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f16x2_t x = {v[2 * i], v[2 * i + 1]};
-    if constexpr (__is_same(E, Bf16))
-      c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x),
-                                          __builtin_bit_cast(bf16x2_t, ones), c, false);
-    else
-      c = __builtin_amdgcn_fdot2(x, ones, c, false);
-  }
+  for (int i = 0; i < 4; ++i) c = sum2<E>(v[2 * i], v[2 * i + 1], c);
   return c;
 }
 // fp32 -> the 16-bit bits of type E (round to nearest even)

@@ -427,8 +427,9 @@ struct SpanCore {
       float p[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) p[j] = exp2_fast(sv[i][j] - m_use);
-      l_run += (p[0] + p[1]) + (p[2] + p[3]);
       pb[i] = to16x4<E>(p[0], p[1], p[2], p[3]);
+      // the sum takes the rounded ones: what multiplies V adds up to one
+      l_run = sum4<E>(pb[i], l_run);
     }
     const unsigned char* vb = stage + (4 * g + (n >> 2)) * C::ROWB + (n & 3) * 8;
     auto vfrag = [&](const unsigned char* at) __attribute__((always_inline)) {

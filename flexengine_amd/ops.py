@@ -60,6 +60,9 @@ class Kv4Pool:
     def device(self) -> torch.device:
         return self.codes.device
 
+    def get_device(self) -> int:
+        return self.codes.get_device()
+
     @property
     def shape(self) -> tuple[int, ...]:
         *lead, hkv, bs, half = self.codes.shape
@@ -84,8 +87,10 @@ def _require_gpu(*tensors: torch.Tensor) -> torch.device:
         raise RuntimeError(
             "flexengine_amd kernels run on a ROCm GPU only; got tensors on " + str(dev)
         )
+    index = dev.index
     for t in tensors[1:]:
-        if t is not None and t.device != dev:
+        # (by number, -1 for the CPU: building a device object per tensor is host time)
+        if t is not None and t.get_device() != index:
             raise ValueError(f"all tensors must be on {dev}; got {t.device}")
     return dev
 
@@ -397,28 +402,32 @@ def _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_
     dev = _require_gpu(q, k_pool, v_pool, block_tables, context_lens, k_new, v_new, out)
     nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     dt = k_pool.dtype
-    if q.ndim != 3 or q.shape[2] != d or q.dtype != dt:
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != d or q.dtype != dt:
         raise ValueError("q must be [batch, num_q_heads, head_dim] of the pools' dtype")
-    batch, hq, _ = q.shape
-    if q.stride(2) != 1 or q.stride(1) != d:
+    batch, hq, _ = shape
+    if stride[2] != 1 or stride[1] != d:
         raise ValueError("q heads must be contiguous")
     if hq % hkv:
         raise ValueError("Q heads must be a multiple of KV heads")
     block_tables = _int32(block_tables, "block_tables")
     context_lens = _int32(context_lens, "context_lens")
-    if block_tables.ndim != 2 or block_tables.shape[0] != batch or context_lens.shape != (batch,):
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != batch or context_lens.shape != (batch,):
         raise ValueError("block_tables must be [batch, W] and context_lens [batch]")
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new must be given together")
     new_stride = 0
     if k_new is not None:
-        if k_new.shape != (batch, hkv, d) or v_new.shape != k_new.shape:
+        shape = (batch, hkv, d)
+        if k_new.shape != shape or v_new.shape != shape:
             raise ValueError("k_new/v_new must be [batch, kv_heads, head_dim]")
         if k_new.dtype != dt or v_new.dtype != dt:
             raise ValueError("k_new/v_new must have the pools' dtype")
-        if k_new.stride() != v_new.stride() or k_new.stride(2) != 1 or k_new.stride(1) != d:
+        stride = k_new.stride()
+        if stride != v_new.stride() or stride[2] != 1 or stride[1] != d:
             raise ValueError("k_new/v_new heads must be contiguous with equal strides")
-        new_stride = k_new.stride(0)
+        new_stride = stride[0]
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != (batch, hq, d) or out.dtype != dt or not out.is_contiguous():
