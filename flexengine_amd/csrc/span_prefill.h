@@ -256,11 +256,13 @@ __device__ __forceinline__ void span_block(const SpanWalk& wk, int t, const unsi
         }
       }
   }
-  float mx = st[0][0];
+  float mx = span_max(st[0][0], st[1][0]), my = span_max(st[0][1], st[1][1]);
 #pragma unroll
-  for (int i = 1; i < 16; ++i) mx = span_max(mx, st[0][i]);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) mx = span_max(mx, st[1][i]);
+  for (int i = 2; i < 16; i += 2) {
+    mx = span_max(span_max(mx, st[0][i]), st[1][i]);
+    my = span_max(span_max(my, st[0][i + 1]), st[1][i + 1]);
+  }
+  mx = span_max(mx, my);
   mx = span_max(mx, other_half(mx, hf)) * scale_log2;
   if (__ballot(mx > r.m + (follow ? kNegInf : kSpanSlack))) {  // wave-uniform
     float m_new = fmaxf(r.m, mx);
@@ -463,9 +465,10 @@ void span_prefill_kernel(const SpanPrefill a) {
   const int nb = wk.blocks();
   int splits = 1;
   if (a.KS > 1 && nb >= kSpanSplitFrom) {
-    // splits of equal shares of the work, so that all of them fit the chip at once: the
-    // units' last ones may be short, at most one more workgroup a unit
-    const int slots = kSpanSlots - work.units * a.Hkv;
+    // splits of equal shares of the work, so that all of them fit the chip at once: the units'
+    // last ones are short, half a workgroup more a unit on average (counted as 5/8: two chunks
+    // of 1000 over up to 4000 cached 71 us, as a whole one 78.5, as 1/2 72.8)
+    const int slots = kSpanSlots - (int)((int64_t)work.units * a.Hkv * 5 / 8);
     if (slots > 0) {
       const int share =
           max((int)(((int64_t)work.blocks * a.Hkv + slots - 1) / slots), kSpanShare);
@@ -593,61 +596,70 @@ void span_prefill_kernel(const SpanPrefill a) {
   __syncthreads();
   if (!last) return;
   if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // thread -> (row, 4 dims); four splits of four rows are read in one round trip
-  constexpr int TPR = D / 4, RPP = NW * kWave / TPR;  // threads a row, rows a pass
-  const int d4 = (int)(threadIdx.x % TPR) * 4;
-  for (int row0 = r0 + (int)threadIdx.x / TPR; row0 <= r_last; row0 += 4 * RPP) {
-    int64_t orow[4];
-    float M[4], den[4];
-    f32x4 num[4];
+  // the splits' weights of every row, then thread -> (row, 4 dims): four splits of six rows are
+  // read in one round trip (four chunks of 256-500 over up to 3000 cached: six rows 46.2 us,
+  // four 47.1, two 49.0, eight, which spills, 47.9; four with every thread's own weights 49.1)
+  float* const weight = reinterpret_cast<float*>(k0);  // [splits][ROWS]
+  static_assert(kSpanMaxSplits * ROWS * sizeof(float) <= sizeof(k0), "weights fit a stage");
+  if ((int)threadIdx.x < ROWS) {
+    const int row = min(r0 + (int)threadIdx.x, r_last);
+    const uint32_t orow = (uint32_t)((u.q0 + row / G) * a.Hq + h * G + row % G);
+    float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = min(row0 + i * RPP, r_last);
-      orow[i] = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
-      M[i] = kNegInf;
-      den[i] = 0.f;
+    for (int s = 0; s < kSpanMaxSplits; ++s) {
+      lv[s] = kNegInf;
+      if (s < splits)
+        lv[s] = __builtin_bit_cast(
+            float, __builtin_amdgcn_raw_buffer_load_b32(
+                       rl, (uint32_t)(s * split_rows + orow) * (uint32_t)sizeof(float), 0, kSpanSc1));
+    }
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s) M = fmaxf(M, lv[s]);
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s) {
+      lv[s] = lv[s] == kNegInf ? 0.f : exp2f(lv[s] - M);
+      den += lv[s];
+    }
+    const float inv_den = den > 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s)
+      if (s < splits) weight[s * ROWS + threadIdx.x] = lv[s] * inv_den;
+  }
+  __syncthreads();
+  constexpr int TPR = D / 4, RPP = NW * kWave / TPR;  // threads a row, rows a pass
+  constexpr int MR = 6;
+  const uint32_t d4 = threadIdx.x % TPR * 4;
+  for (int row0 = (int)threadIdx.x / TPR; r0 + row0 <= r_last; row0 += MR * RPP) {
+    uint32_t orow[MR];
+    f32x4 num[MR];
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      const int row = min(r0 + row0 + i * RPP, r_last);
+      orow[i] = (uint32_t)((u.q0 + row / G) * a.Hq + h * G + row % G);
       num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int s0 = 0; s0 < splits; s0 += 4) {
-      float lv[4][4];
-      f32x4 ov[4][4];
+      f32x4 ov[MR][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 4; ++k)
+        if (s0 + k < splits)  // workgroup-uniform
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int s = s0 + k < splits ? s0 + k : splits - 1;
-          const uint32_t prow = (uint32_t)(s * split_rows + orow[i]);
-          lv[i][k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                                   rl, prow * (uint32_t)sizeof(float), 0, kSpanSc1));
-          ov[i][k] = __builtin_bit_cast(
-              f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                         ro, (prow * D + d4) * (uint32_t)sizeof(float), 0, kSpanSc1));
-        }
+          for (int i = 0; i < MR; ++i)
+            ov[i][k] = __builtin_bit_cast(
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                           ro, ((uint32_t)((s0 + k) * split_rows + orow[i]) * D + d4) *
+                                   (uint32_t)sizeof(float), 0, kSpanSc1));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float bm = M[i];
+      for (int k = 0; k < 4; ++k)
+        if (s0 + k < splits)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (s0 + k >= splits) lv[i][k] = kNegInf;
-          bm = fmaxf(bm, lv[i][k]);
-        }
-        const float alpha = M[i] == kNegInf ? 0.f : exp2f(M[i] - bm);
-        num[i] *= alpha;
-        den[i] *= alpha;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float wt = lv[i][k] == kNegInf ? 0.f : exp2f(lv[i][k] - bm);
-          num[i] += wt * ov[i][k];
-          den[i] += wt;
-        }
-        M[i] = bm;
-      }
+          for (int i = 0; i < MR; ++i)
+            num[i] += weight[(s0 + k) * ROWS + min(row0 + i * RPP, ROWS - 1)] * ov[i][k];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (row0 + i * RPP <= r_last && (!PAD || d4 < DR))
-        *reinterpret_cast<f16x4*>(a.out + orow[i] * DR + d4) =
-            to16x4<E>(num[i] * (den[i] > 0.f ? 1.f / den[i] : 0.f));
+    for (int i = 0; i < MR; ++i)
+      if (r0 + row0 + i * RPP <= r_last && (!PAD || (int)d4 < DR))
+        *reinterpret_cast<f16x4*>(a.out + (int64_t)orow[i] * DR + d4) = to16x4<E>(num[i]);
   }
 }
 

@@ -7,31 +7,34 @@ namespace {
 
 // ---- fp32 pools ---------------------------------------------------------------------------
 // The plain fp32 prefill's organisation on the same engine (F32Core, attn_core.h): a workgroup
-// takes 16 * RT rows of a sequence and KV head, its four waves the row block's 16-key tiles in
-// turn -- the tiles of the sinks and those from the first row's window start on -- and the
-// waves' states are joined in LDS.  Bound by the fp32 MFMAs (154 TFLOP/s in a large product).
+// takes 16 rows of a sequence and KV head, its four waves the row block's 16-key tiles in turn
+// -- the tiles of the sinks and those from the first row's window start on -- and the waves'
+// states are joined in LDS.  Bound by the fp32 MFMAs (154 TFLOP/s in a large product): three
+// chunks of 100-700 tokens of 12/2 heads under a window of 512 40.9 us, 65 TFLOP/s, half the
+// chip in its second round.  32 rows a workgroup, which halve the reads of K and V: 49.1 us,
+// and four chunks of 500 under 1024 120 -> 145; eight waves 50.5.
 constexpr int kF32Waves = 4;
 
-template <int D, int RT>
+template <int D>
 struct SpanF32Lds {
   static constexpr int NX = D / 16;
-  static constexpr size_t park = 0;  // [kF32Waves][RT * NX][64] x 16 bytes
-  static constexpr size_t park_m = park + (size_t)kF32Waves * RT * NX * kWave * 16;
-  static constexpr size_t park_l = park_m + (size_t)kF32Waves * RT * kWave * sizeof(float);
-  static constexpr size_t bytes = park_l + (size_t)kF32Waves * RT * kWave * sizeof(float);
+  static constexpr size_t park = 0;  // [kF32Waves][NX][64] x 16 bytes
+  static constexpr size_t park_m = park + (size_t)kF32Waves * NX * kWave * 16;
+  static constexpr size_t park_l = park_m + (size_t)kF32Waves * kWave * sizeof(float);
+  static constexpr size_t bytes = park_l + (size_t)kF32Waves * kWave * sizeof(float);
 };
 
-template <int D, bool PAD, int RT>
-__global__ __launch_bounds__(kF32Waves* kWave)
-__attribute__((amdgpu_waves_per_eu(RT == 1 ? 3 : 2, 8)))
+template <int D, bool PAD>
+__global__ __launch_bounds__(kF32Waves* kWave) __attribute__((amdgpu_waves_per_eu(3, 8)))
 void span_prefill_f32_kernel(const SpanPrefill a) {
-  using Core = F32Core<D, true, PAD, RT, true>;
-  using Lds = SpanF32Lds<D, RT>;
-  constexpr int ROWS = 16 * RT;
+  using Core = F32Core<D, true, PAD, 1, true>;
+  using Lds = SpanF32Lds<D>;
+  constexpr int ROWS = kTile;
   constexpr int NX = Core::NX;
   extern __shared__ __align__(16) unsigned char smem[];
   const int DR = PAD ? a.dr : D;
   const int h = blockIdx.x % a.Hkv;
+  // the later units, which see more keys, first
   const int item = (int)gridDim.x / a.Hkv - 1 - (int)blockIdx.x / a.Hkv;
   SpanUnit u;
   SpanWork work;
@@ -46,6 +49,9 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   const int cached = ctx >= u.n ? ctx - u.n : 0;
   const int r0 = u.block * ROWS;
   const int r_last = min(r0 + ROWS, total_rows) - 1;
+  const int row = r0 + n;
+  const bool valid = row < total_rows;
+  const int rc = valid ? row : r_last;
 
   Core core;
   core.k_pool = (const float*)a.k_pool;
@@ -60,32 +66,26 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   core.NB = a.NB;
   core.BS = a.BS;
   core.bs_log2 = a.bs_log2;
-  core.tok_end = cached + r_last / G + 1;
   core.scale_log2 = a.scale_log2;
   core.knew_row = nullptr;
   core.vnew_row = nullptr;
   core.new_pos = -1;
-  core.sinks = a.span.sinks;
-  core.wmin = window_start(a.span, cached + r0 / G);
-  core.span_head = (int)(((unsigned)a.span.sinks + kTile - 1) / kTile);
-  core.span_skip = span_skip(a.span, core.wmin, kTile);
-  const int ntiles =
-      core.begin(w, kF32Waves, (core.tok_end + kTile - 1) / kTile - core.span_skip);
+  SpanWalk wk;
+  wk.init(a.span, cached + r0 / G, cached + r_last / G);
+  core.tok_end = wk.key_end;
+  core.sinks = wk.sinks;
+  core.wmin = wk.ws;
+  core.span_head = wk.head;
+  core.span_skip = wk.skip;
+  core.limit[0] = valid ? cached + rc / G + 1 : 0;
+  core.wlo[0] = window_start(a.span, cached + rc / G);
+  const int ntiles = core.begin(w, kF32Waves, (wk.key_end + kTile - 1) / kTile - wk.skip);
+  const float* qrow = (const float*)a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = r0 + 16 * rt + n;
-    const bool valid = row < total_rows;
-    const int rc = valid ? row : r_last;
-    core.limit[rt] = valid ? cached + rc / G + 1 : 0;
-    core.wlo[rt] = window_start(a.span, cached + rc / G);
-    const float* qrow =
-        (const float*)a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR;
-#pragma unroll
-    for (int c = 0; c < Core::NC; ++c) {
-      core.qv[rt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (!PAD || 16 * c + 4 * g < DR)
-        core.qv[rt][c] = *reinterpret_cast<const f32x4*>(qrow + 16 * c + 4 * g);
-    }
+  for (int c = 0; c < Core::NC; ++c) {
+    core.qv[0][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!PAD || 16 * c + 4 * g < DR)
+      core.qv[0][c] = *reinterpret_cast<const f32x4*>(qrow + 16 * c + 4 * g);
   }
   core.init_acc();
   core.run_single(ntiles);
@@ -94,52 +94,39 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   float* park_m = reinterpret_cast<float*>(smem + Lds::park_m);
   float* park_l = reinterpret_cast<float*>(smem + Lds::park_l);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-    for (int x = 0; x < NX; ++x) park[((w * RT + rt) * NX + x) * kWave + lane] = core.o[rt][x];
-    park_m[(w * RT + rt) * kWave + lane] = core.m_run[rt];
-    park_l[(w * RT + rt) * kWave + lane] = core.l_total(rt);
-  }
+  for (int x = 0; x < NX; ++x) park[(w * NX + x) * kWave + lane] = core.o[0][x];
+  park_m[w * kWave + lane] = core.m_run[0];
+  park_l[w * kWave + lane] = core.l_total();
   __syncthreads();
-  for (int t = w; t < RT * NX; t += kF32Waves) {
-    const int rt = t / NX, x = t % NX;
-    const int row = r0 + 16 * rt + n;
-    float M = kNegInf;
+  float M = kNegInf, den = 0.f, sc[kF32Waves];
 #pragma unroll
-    for (int v = 0; v < kF32Waves; ++v) M = fmaxf(M, park_m[(v * RT + rt) * kWave + lane]);
-    float den = 0.f;
+  for (int v = 0; v < kF32Waves; ++v) M = fmaxf(M, park_m[v * kWave + lane]);
+#pragma unroll
+  for (int v = 0; v < kF32Waves; ++v) {
+    const float mv = park_m[v * kWave + lane];
+    sc[v] = mv == kNegInf ? 0.f : exp2f(mv - M);
+    den += sc[v] * park_l[v * kWave + lane];
+  }
+  if (!valid) return;
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const int64_t orow = ((int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G) * DR;
+  for (int x = w; x < NX; x += kF32Waves) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < kF32Waves; ++v) {
-      const float mv = park_m[(v * RT + rt) * kWave + lane];
-      const float sc = mv == kNegInf ? 0.f : exp2f(mv - M);
-      den += sc * park_l[(v * RT + rt) * kWave + lane];
+    for (int v = 0; v < kF32Waves; ++v)
       // tile x as the 16 dims from 16 x (a lane parked its 4 dims from f32_dim0)
-      acc += sc * park[((v * RT + rt) * NX + (x & ~3) + g) * kWave + 16 * (x & 3) + n];
-    }
-    if (row >= total_rows) continue;
-    const float inv = den > 0.f ? 1.f / den : 0.f;
-    const int64_t r = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
+      acc += sc[v] * park[(v * NX + (x & ~3) + g) * kWave + 16 * (x & 3) + n];
     const int d0 = 16 * x + 4 * g;
-    if (!PAD || d0 < DR) store_out4<F32>(a.out, r * DR + d0, acc * inv);
+    if (!PAD || d0 < DR) store_out4<F32>(a.out, orow + d0, acc * inv);
   }
 }
 
 template <int D, bool PAD>
 int launch_f32(const SpanPrefill& a, hipStream_t s) {
-  // two row tiles halve the K/V reads per product, and the workgroups (the plain fp32
-  // prefill's rule and figures: prefill.hip)
-  const int64_t rows = (int64_t)a.total_q * a.G;
-  const int rt = rows * a.Hkv >= 20480 && rows >= (int64_t)48 * a.S ? 2 : 1;
-  const int64_t units = (rows + 16 * rt - 1) / (16 * rt) + a.S;
+  const int64_t units = ((int64_t)a.total_q * a.G + kTile - 1) / kTile + a.S;
   if (units * a.Hkv >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)(units * a.Hkv)), block(kF32Waves * kWave);
-  if (rt == 2)
-    hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD, 2>), grid, block, (SpanF32Lds<D, 2>::bytes),
-                       s, a);
-  else
-    hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD, 1>), grid, block, (SpanF32Lds<D, 1>::bytes),
-                       s, a);
+  hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD>), dim3((unsigned)(units * a.Hkv)),
+                     dim3(kF32Waves * kWave), SpanF32Lds<D>::bytes, s, a);
   return FE_LAUNCH_STATUS();
 }
 
