@@ -52,10 +52,10 @@ constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
 constexpr int kSpanSc1 = 16;       // buffer-instruction cache policy: sc1 (device-coherent)
 // Blocks of a walk over which the reference of the softmax follows every block's maximum in
 // either direction (the probabilities' rounding is then relative to the block's own largest);
-// after them it lags by up to kRescaleSlack.  With a slack of 2, as the wide 16-bit prefill has
-// for the last percent of accuracy, 4095 tokens over a 4-bit cache took 148 instead of 142 us
-// and 8191 under a window of 1024 168 instead of 164; the error against 64 bits (bf16) was
-// 2.0e-3 and 2.1e-3 instead of 1.9e-3 and 2.0e-3 (1.6e-3 is the output type's own).
+// after them it lags by up to kRescaleSlack.  4095 tokens over a 4-bit cache, 8191 under a
+// window of 1024 (bf16): 142 and 164 us, 2.0e-3 and 2.1e-3 from 64 bits (the output's rounding
+// alone is 1.6e-3); with a slack of 2, as the wide 16-bit prefill has, 148 and 168 us, 1.9e-3
+// and 2.0e-3.
 constexpr int kSpanFollow = 2;
 
 struct SpanPrefill {
@@ -231,10 +231,12 @@ __device__ __forceinline__ void span_block(const SpanWalk& wk, int t, const unsi
         f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((span_lds_s16x4*)(vb + 8 * C::ROWB + slot)));
     return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   };
-  // the first 32 keys' V fragments are read before the softmax, which hides their latency
-  f16x8 vf[2][NT];
+  // the first 32 keys' V fragments are read before the softmax, which hides their latency (16
+  // keys' at D = 256, for registers)
+  constexpr int VS = D > 128 ? 1 : 2;
+  f16x8 vf[VS][NT];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < VS; ++s)
 #pragma unroll
     for (int x = 0; x < NT; ++x) vf[s][x] = vfrag(s, x);
 
@@ -290,8 +292,9 @@ __device__ __forceinline__ void span_block(const SpanWalk& wk, int t, const unsi
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-      const f16x8 va = vf[s % 2][x];
-      if (s < 2) vf[s][x] = vfrag(s + 2, x);  // in flight during the next 16 keys' products
+      const f16x8 va = vf[s % VS][x];
+      // in flight during the products before its own
+      if (s + VS < 4) vf[s % VS][x] = vfrag(s + VS, x);
       r.o[x] = mma32x32<E>(va, pb[s], r.o[x]);
     }
 }
