@@ -47,6 +47,7 @@ constexpr int kSpanSlots = 512;
 constexpr int kSpanSplitFrom = 12;
 constexpr int kSpanShare = 6;
 constexpr int kSpanMaxSplits = 16;
+typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSpanTickets = 65536;
 constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
 constexpr int kSpanSc1 = 16;       // buffer-instruction cache policy: sc1 (device-coherent)
@@ -130,7 +131,9 @@ __device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUn
       SpanWalk f, l;
       f.init(a.span, cached, cached + step - 1);
       l.init(a.span, cached + n - step, cached + n - 1);
-      work.blocks += wave_sum_i(n > 0 ? (f.blocks() + l.blocks()) * nb / 2 : 0);
+      const int64_t walked = (int64_t)(f.blocks() + l.blocks()) * nb / 2;
+      // (bounded: split units are few, and KS bounds their splits)
+      work.blocks += wave_sum_i(n > 0 ? (int)min(walked, (int64_t)1 << 20) : 0);
     }
     const int incl = wave_scan_incl_i(nb) + carry;
     const unsigned long long hit = __ballot(item >= incl - nb && item < incl);
@@ -148,6 +151,131 @@ __device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUn
   }
   work.units = carry;
   return found;
+}
+
+// ---- key splits -----------------------------------------------------------------------------
+
+// Splits of a unit of nb key blocks
+__device__ __forceinline__ int span_splits(const SpanPrefill& a, const SpanWork& work, int nb,
+                                           int chip) {
+  if (a.KS == 1 || nb < kSpanSplitFrom) return 1;
+  // equal shares of the work, so that all splits fit the chip at once: the units' last ones are
+  // short, half a workgroup more a unit on average (counted as 5/8: two chunks of 1000 over up
+  // to 4000 cached 71 us, as a whole one 78.5, as 1/2 72.8)
+  const int slots = chip - (int)((int64_t)work.units * a.Hkv * 5 / 8);
+  if (slots <= 0) return 1;
+  const int share = max((int)(((int64_t)work.blocks * a.Hkv + slots - 1) / slots), kSpanShare);
+  return min((nb + share - 1) / share, a.KS);
+}
+
+// The splits' rows: normalised fp32 outputs [KS][total_q * Hq][D] and base-2 log-sum-exps,
+// device-coherent (the host keeps them under 2 GiB)
+struct SplitRows {
+  __amdgpu_buffer_rsrc_t ro, rl;
+  int64_t rows;  // of a split
+  int D;
+  __device__ __forceinline__ SplitRows(const SpanPrefill& a, int d) {
+    rows = (int64_t)a.total_q * a.Hq;
+    D = d;
+    ro = __builtin_amdgcn_make_buffer_rsrc(a.part_o, 0, (int)(a.KS * rows * D * 4), 0x00020000);
+    rl = __builtin_amdgcn_make_buffer_rsrc(a.part_lse, 0, (int)(a.KS * rows * 4), 0x00020000);
+  }
+  __device__ __forceinline__ uint32_t at(int s, int64_t row) const {
+    return (uint32_t)(s * rows + row);
+  }
+  __device__ __forceinline__ void store(int s, int64_t row, int d0, f32x4 v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(span_u32x4, v), ro,
+                                           (at(s, row) * D + d0) * (uint32_t)sizeof(float), 0,
+                                           kSpanSc1);
+  }
+  __device__ __forceinline__ f32x4 load(int s, int64_t row, int d0) const {
+    return __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                   ro, (at(s, row) * D + d0) * (uint32_t)sizeof(float), 0, kSpanSc1));
+  }
+  __device__ __forceinline__ void store_lse(int s, int64_t row, float v) const {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rl,
+                                          at(s, row) * (uint32_t)sizeof(float), 0, kSpanSc1);
+  }
+  __device__ __forceinline__ float load_lse(int s, int64_t row) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                         rl, at(s, row) * (uint32_t)sizeof(float), 0, kSpanSc1));
+  }
+};
+
+// Whether this workgroup is the unit's last: its rows are complete before its ticket is drawn,
+// and the last one sets the ticket back to zero.
+__device__ __forceinline__ bool last_split(int* ticket, int splits, int* last) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows are complete
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+            splits - 1;
+  __syncthreads();
+  if (!*last) return false;
+  if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
+}
+
+// Joins the splits of a unit's rows 0 .. r_last (row_of: their output rows) by T threads: the
+// splits' weights of every row into LDS (weight [splits][ROWS]), then thread -> (row, 4 dims),
+// four splits of MR rows in one round trip.  Four chunks of 256-500 over up to 3000 cached: six
+// rows 46.2 us, four 47.1, two 49.0, eight, which spills, 47.9; four with every thread's own
+// weights 49.1.
+template <class E, int D, bool PAD, int ROWS, int T, int MR, class RowOf>
+__device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRows& part, int splits,
+                                            float* weight, int r_last, RowOf row_of) {
+  if ((int)threadIdx.x < ROWS) {
+    const uint32_t orow = row_of(min((int)threadIdx.x, r_last));
+    float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s) {
+      lv[s] = kNegInf;
+      if (s < splits) lv[s] = part.load_lse(s, orow);
+    }
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s) M = fmaxf(M, lv[s]);
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s) {
+      lv[s] = lv[s] == kNegInf ? 0.f : exp2f(lv[s] - M);
+      den += lv[s];
+    }
+    const float inv = den > 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int s = 0; s < kSpanMaxSplits; ++s)
+      if (s < splits) weight[s * ROWS + threadIdx.x] = lv[s] * inv;
+  }
+  __syncthreads();
+  constexpr int TPR = D / 4, RPP = T / TPR;  // threads a row, rows a pass
+  const int DR = PAD ? a.dr : D;
+  const int d4 = (int)(threadIdx.x % TPR) * 4;
+  for (int row0 = (int)threadIdx.x / TPR; row0 <= r_last; row0 += MR * RPP) {
+    uint32_t orow[MR];
+    f32x4 num[MR];
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      orow[i] = row_of(min(row0 + i * RPP, r_last));
+      num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+      f32x4 ov[MR][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s0 + k < splits)  // workgroup-uniform
+#pragma unroll
+          for (int i = 0; i < MR; ++i) ov[i][k] = part.load(s0 + k, orow[i], d4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s0 + k < splits)
+#pragma unroll
+          for (int i = 0; i < MR; ++i)
+            num[i] += weight[(s0 + k) * ROWS + min(row0 + i * RPP, ROWS - 1)] * ov[i][k];
+    }
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+      if (row0 + i * RPP <= r_last && (!PAD || d4 < DR))
+        store_out4<E>(a.out, (int64_t)orow[i] * DR + d4, num[i]);
+  }
 }
 
 template <int D, bool Q4>
@@ -175,7 +303,6 @@ __device__ __forceinline__ float other_half(float x, int hf) {
 
 typedef __attribute__((address_space(3))) void span_lds_void;
 typedef __attribute__((address_space(3))) s16x4 span_lds_s16x4;
-typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t span_rsrc(const void* base, uint32_t bytes) {
   const uint64_t addr = reinterpret_cast<uint64_t>(base);
@@ -465,18 +592,7 @@ void span_prefill_kernel(const SpanPrefill a) {
   SpanWalk wk;
   wk.init(a.span, cached + r0 / G, cached + r_last / G);
   const int nb = wk.blocks();
-  int splits = 1;
-  if (a.KS > 1 && nb >= kSpanSplitFrom) {
-    // splits of equal shares of the work, so that all of them fit the chip at once: the units'
-    // last ones are short, half a workgroup more a unit on average (counted as 5/8: two chunks
-    // of 1000 over up to 4000 cached 71 us, as a whole one 78.5, as 1/2 72.8)
-    const int slots = kSpanSlots - (int)((int64_t)work.units * a.Hkv * 5 / 8);
-    if (slots > 0) {
-      const int share =
-          max((int)(((int64_t)work.blocks * a.Hkv + slots - 1) / slots), kSpanShare);
-      splits = min((nb + share - 1) / share, a.KS);
-    }
-  }
+  const int splits = span_splits(a, work, nb, kSpanSlots);
   if (ks >= splits) return;
   const int j0 = (int)((int64_t)nb * ks / splits), j1 = (int)((int64_t)nb * (ks + 1) / splits);
 
@@ -566,103 +682,25 @@ void span_prefill_kernel(const SpanPrefill a) {
     return;
   }
 
-  // ---- the split's rows, and the join by the unit's last split (the host keeps the partials
-  // under 2 GiB) ----
-  const int64_t split_rows = (int64_t)a.total_q * a.Hq;
-  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
-      a.part_o, 0, (int)(a.KS * split_rows * D * 4), 0x00020000);
-  const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(
-      a.part_lse, 0, (int)(a.KS * split_rows * 4), 0x00020000);
+  const SplitRows part(a, D);
   if (valid) {
-    const uint32_t prow = (uint32_t)(ks * split_rows + (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G);
+    const int64_t orow = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const f32x4 t = {r.o[x][4 * q4], r.o[x][4 * q4 + 1], r.o[x][4 * q4 + 2], r.o[x][4 * q4 + 3]};
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(span_u32x4, t * inv), ro,
-            (prow * D + 32 * x + 8 * q4 + 4 * hf) * (uint32_t)sizeof(float), 0, kSpanSc1);
+        part.store(ks, orow, 32 * x + 8 * q4 + 4 * hf, t * inv);
       }
-    if (hf == 0)
-      __builtin_amdgcn_raw_buffer_store_b32(
-          __builtin_bit_cast(uint32_t, l > 0.f ? r.m + log2f(l) : kNegInf), rl,
-          prow * (uint32_t)sizeof(float), 0, kSpanSc1);
+    if (hf == 0) part.store_lse(ks, orow, l > 0.f ? r.m + log2f(l) : kNegInf);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows are complete
-  __syncthreads();
-  int* const ticket = a.tickets + item * a.Hkv + h;
-  if (threadIdx.x == 0)
-    last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-           splits - 1;
-  __syncthreads();
-  if (!last) return;
-  if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the splits' weights of every row, then thread -> (row, 4 dims): four splits of six rows are
-  // read in one round trip (four chunks of 256-500 over up to 3000 cached: six rows 46.2 us,
-  // four 47.1, two 49.0, eight, which spills, 47.9; four with every thread's own weights 49.1)
-  float* const weight = reinterpret_cast<float*>(k0);  // [splits][ROWS]
+  if (!last_split(a.tickets + item * a.Hkv + h, splits, &last)) return;
   static_assert(kSpanMaxSplits * ROWS * sizeof(float) <= sizeof(k0), "weights fit a stage");
-  if ((int)threadIdx.x < ROWS) {
-    const int row = min(r0 + (int)threadIdx.x, r_last);
-    const uint32_t orow = (uint32_t)((u.q0 + row / G) * a.Hq + h * G + row % G);
-    float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) {
-      lv[s] = kNegInf;
-      if (s < splits)
-        lv[s] = __builtin_bit_cast(
-            float, __builtin_amdgcn_raw_buffer_load_b32(
-                       rl, (uint32_t)(s * split_rows + orow) * (uint32_t)sizeof(float), 0, kSpanSc1));
-    }
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) M = fmaxf(M, lv[s]);
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) {
-      lv[s] = lv[s] == kNegInf ? 0.f : exp2f(lv[s] - M);
-      den += lv[s];
-    }
-    const float inv_den = den > 0.f ? 1.f / den : 0.f;
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s)
-      if (s < splits) weight[s * ROWS + threadIdx.x] = lv[s] * inv_den;
-  }
-  __syncthreads();
-  constexpr int TPR = D / 4, RPP = NW * kWave / TPR;  // threads a row, rows a pass
-  constexpr int MR = 6;
-  const uint32_t d4 = threadIdx.x % TPR * 4;
-  for (int row0 = (int)threadIdx.x / TPR; r0 + row0 <= r_last; row0 += MR * RPP) {
-    uint32_t orow[MR];
-    f32x4 num[MR];
-#pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      const int row = min(r0 + row0 + i * RPP, r_last);
-      orow[i] = (uint32_t)((u.q0 + row / G) * a.Hq + h * G + row % G);
-      num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int s0 = 0; s0 < splits; s0 += 4) {
-      f32x4 ov[MR][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (s0 + k < splits)  // workgroup-uniform
-#pragma unroll
-          for (int i = 0; i < MR; ++i)
-            ov[i][k] = __builtin_bit_cast(
-                f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                           ro, ((uint32_t)((s0 + k) * split_rows + orow[i]) * D + d4) *
-                                   (uint32_t)sizeof(float), 0, kSpanSc1));
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (s0 + k < splits)
-#pragma unroll
-          for (int i = 0; i < MR; ++i)
-            num[i] += weight[(s0 + k) * ROWS + min(row0 + i * RPP, ROWS - 1)] * ov[i][k];
-    }
-#pragma unroll
-    for (int i = 0; i < MR; ++i)
-      if (r0 + row0 + i * RPP <= r_last && (!PAD || (int)d4 < DR))
-        *reinterpret_cast<f16x4*>(a.out + (int64_t)orow[i] * DR + d4) = to16x4<E>(num[i]);
-  }
+  join_splits<E, D, PAD, ROWS, NW * kWave, 6>(
+      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0,
+      [&](int i) __attribute__((always_inline)) {
+        return (uint32_t)((u.q0 + (r0 + i) / G) * a.Hq + h * G + (r0 + i) % G);
+      });
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -696,15 +734,18 @@ inline int span_waves(int num_seqs, int total_q, int hq, int hkv, int d, int win
              ? 8
              : 4;
 }
-inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d, int window, bool q4) {
+// rows of a unit (0: 32 a wave) and workgroups that run at once: the 16-bit kernel's, unless given
+inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d, int window, bool q4,
+                            int unit_rows = 0, int chip = kSpanSlots) {
   SpanShape p;
   const int64_t rows = (int64_t)total_q * (hq / hkv);
   p.waves = span_waves(num_seqs, total_q, hq, hkv, d, window, q4);
-  p.units = (rows + 32 * p.waves - 1) / (32 * p.waves) + num_seqs;
+  if (unit_rows == 0) unit_rows = 32 * p.waves;
+  p.units = (rows + unit_rows - 1) / unit_rows + num_seqs;
   // key splits of a unit at most: twice the slots over the units, for those with more keys
   // than the others
-  const int64_t wgs = ((rows + 32 * p.waves - 1) / (32 * p.waves)) * hkv;
-  int64_t ks = wgs > 0 ? 2 * kSpanSlots / wgs : 1;
+  const int64_t wgs = ((rows + unit_rows - 1) / unit_rows) * hkv;
+  int64_t ks = wgs > 0 ? 2 * chip / wgs : 1;
   ks = ks < 1 ? 1 : (ks > kSpanMaxSplits ? kSpanMaxSplits : ks);
   if (p.waves != 4 || p.units * hkv > kSpanTickets) ks = 1;
   const int64_t part_rows = (int64_t)total_q * hq;

@@ -12,8 +12,12 @@ namespace {
 // states are joined in LDS.  Bound by the fp32 MFMAs (154 TFLOP/s in a large product): three
 // chunks of 100-700 tokens of 12/2 heads under a window of 512 40.9 us, 65 TFLOP/s, half the
 // chip in its second round.  32 rows a workgroup, which halve the reads of K and V: 49.1 us,
-// and four chunks of 500 under 1024 120 -> 145; eight waves 50.5.
+// and four chunks of 500 under 1024 120 -> 145; eight waves 50.5.  Units too few for the chip
+// share their keys out over splits, as the 16-bit kernel's do (span_prefill.h): 50 tokens over up
+// to 3000 under a window of 2000 38.3 -> 18.6 us, four chunks of 10-20 over up to 8000 under 4000
+// 92.6 -> 37.3 (four chunks of 500 at head_dim 96, not split, 128.5 -> 133 for its registers).
 constexpr int kF32Waves = 4;
+constexpr int kF32Slots = 768;  // workgroups that run at once: three on each of 256 CUs
 
 template <int D>
 struct SpanF32Lds {
@@ -21,7 +25,8 @@ struct SpanF32Lds {
   static constexpr size_t park = 0;  // [kF32Waves][NX][64] x 16 bytes
   static constexpr size_t park_m = park + (size_t)kF32Waves * NX * kWave * 16;
   static constexpr size_t park_l = park_m + (size_t)kF32Waves * kWave * sizeof(float);
-  static constexpr size_t bytes = park_l + (size_t)kF32Waves * kWave * sizeof(float);
+  static constexpr size_t last = park_l + (size_t)kF32Waves * kWave * sizeof(float);
+  static constexpr size_t bytes = last + sizeof(int);
 };
 
 template <int D, bool PAD>
@@ -34,8 +39,10 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int DR = PAD ? a.dr : D;
   const int h = blockIdx.x % a.Hkv;
-  // the later units, which see more keys, first
-  const int item = (int)gridDim.x / a.Hkv - 1 - (int)blockIdx.x / a.Hkv;
+  // by split, then the later units, which see more keys, first
+  const int items = (int)gridDim.x / (a.Hkv * a.KS);
+  const int ks = (int)blockIdx.x / a.Hkv / items;
+  const int item = items - 1 - (int)blockIdx.x / a.Hkv % items;
   SpanUnit u;
   SpanWork work;
   if (!find_unit<ROWS>(a, item, u, work)) return;
@@ -79,7 +86,11 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   core.span_skip = wk.skip;
   core.limit[0] = valid ? cached + rc / G + 1 : 0;
   core.wlo[0] = window_start(a.span, cached + rc / G);
-  const int ntiles = core.begin(w, kF32Waves, (wk.key_end + kTile - 1) / kTile - wk.skip);
+  const int nt = (wk.key_end + kTile - 1) / kTile - wk.skip;
+  const int splits = span_splits(a, work, wk.blocks(), kF32Slots);
+  if (ks >= splits) return;
+  const int ntiles = core.begin((int)((int64_t)nt * ks / splits) + w, kF32Waves,
+                                (int)((int64_t)nt * (ks + 1) / splits));
   const float* qrow = (const float*)a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR;
 #pragma unroll
   for (int c = 0; c < Core::NC; ++c) {
@@ -107,9 +118,9 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
     sc[v] = mv == kNegInf ? 0.f : exp2f(mv - M);
     den += sc[v] * park_l[v * kWave + lane];
   }
-  if (!valid) return;
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  const int64_t orow = ((int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G) * DR;
+  const int64_t orow = (int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G;
+  const SplitRows part(a, D);
   for (int x = w; x < NX; x += kF32Waves) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -117,15 +128,28 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
       // tile x as the 16 dims from 16 x (a lane parked its 4 dims from f32_dim0)
       acc += sc[v] * park[(v * NX + (x & ~3) + g) * kWave + 16 * (x & 3) + n];
     const int d0 = 16 * x + 4 * g;
-    if (!PAD || d0 < DR) store_out4<F32>(a.out, orow + d0, acc * inv);
+    if (!valid) continue;
+    if (splits > 1)
+      part.store(ks, orow, d0, acc * inv);
+    else if (!PAD || d0 < DR)
+      store_out4<F32>(a.out, orow * DR + d0, acc * inv);
   }
+  if (splits == 1) return;
+  if (valid && w == 0 && g == 0) part.store_lse(ks, orow, den > 0.f ? M + log2f(den) : kNegInf);
+  int* const last = reinterpret_cast<int*>(smem + Lds::last);
+  if (!last_split(a.tickets + item * a.Hkv + h, splits, last)) return;
+  join_splits<F32, D, PAD, ROWS, kF32Waves * kWave, 2>(
+      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0,
+      [&](int r) __attribute__((always_inline)) {
+        return (uint32_t)((u.q0 + (r0 + r) / G) * a.Hq + h * G + (r0 + r) % G);
+      });
 }
 
 template <int D, bool PAD>
 int launch_f32(const SpanPrefill& a, hipStream_t s) {
   const int64_t units = ((int64_t)a.total_q * a.G + kTile - 1) / kTile + a.S;
-  if (units * a.Hkv >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD>), dim3((unsigned)(units * a.Hkv)),
+  if (units * a.Hkv * a.KS >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD>), dim3((unsigned)(units * a.Hkv * a.KS)),
                      dim3(kF32Waves * kWave), SpanF32Lds<D>::bytes, s, a);
   return FE_LAUNCH_STATUS();
 }
@@ -133,7 +157,8 @@ int launch_f32(const SpanPrefill& a, hipStream_t s) {
 int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v_pool,
                      int num_blocks, const int32_t* tables, int table_stride, const int32_t* q_off,
                      const int32_t* ctx, int num_seqs, int total_q, int hq, int hkv, int d, int bs,
-                     float scale, int window, int sinks, fe_stream_t stream) {
+                     float scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                     fe_stream_t stream) {
   FE_CHECK_ARG(num_seqs >= 0 && total_q >= 0 && hq > 0 && hkv > 0 && d > 0 && num_blocks > 0 &&
                table_stride > 0 && window > 0 && sinks >= 0 && hq % hkv == 0 && scale > 0.f);
   const int bs_log2 = span_log2(bs);
@@ -146,7 +171,13 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
   FE_CHECK_ARG(q && out && k_pool && v_pool && tables && q_off && ctx);
   const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
+  const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d, window, false, kTile, kF32Slots);
+  if (workspace == nullptr || workspace_bytes < p.bytes || !aligned(workspace))
+    return FE_ERR_WORKSPACE;
   SpanPrefill a{};
+  a.tickets = (int*)workspace;
+  a.part_o = (float*)((char*)workspace + p.o);
+  a.part_lse = (float*)((char*)workspace + p.lse);
   a.q = (const f16*)q;
   a.out = (f16*)out;
   a.k_pool = k_pool;
@@ -163,7 +194,7 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
   a.BS = bs;
   a.bs_log2 = bs_log2;
   a.NB = num_blocks;
-  a.KS = 1;
+  a.KS = p.ks;
   a.dr = d;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, sinks};
@@ -181,7 +212,10 @@ extern "C" size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int 
       num_q_heads % kv_heads)
     return 0;
   // (the form of eight waves takes no more)
-  return span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim, 1, false).bytes;
+  const size_t b16 = span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim, 1, false).bytes;
+  const size_t b32 = span_shape(num_seqs, total_q, num_q_heads, kv_heads, head_dim, 1, false, kTile,
+                                kF32Slots).bytes;
+  return b16 > b32 ? b16 : b32;
 }
 
 #define FE_WINDOW_PREFILL(SUFFIX, E)                                                              \
@@ -205,9 +239,10 @@ extern "C" int fe_prefill_paged_window_f32(const void* q, void* out, const void*
                                            const int32_t* q_offsets, const int32_t* context_lens,
                                            int num_seqs, int total_q, int num_q_heads,
                                            int kv_heads, int head_dim, int block_size, float scale,
-                                           int window, int sinks, void*, size_t,
-                                           fe_stream_t stream) {
+                                           int window, int sinks, void* workspace,
+                                           size_t workspace_bytes, fe_stream_t stream) {
   return span_prefill_f32(q, out, k_pool, v_pool, num_blocks, block_tables, table_stride,
                           q_offsets, context_lens, num_seqs, total_q, num_q_heads, kv_heads,
-                          head_dim, block_size, scale, window, sinks, stream);
+                          head_dim, block_size, scale, window, sinks, workspace, workspace_bytes,
+                          stream);
 }

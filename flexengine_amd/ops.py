@@ -719,16 +719,15 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no prefill plan")
-        if workspace is None and q.dtype != FP32:
+        if workspace is None:
             workspace = decode_workspace(dev, int(_lib.load().fe_span_prefill_workspace_size(
                 num_seqs, total_q, hq, hkv, d)), kind="span_prefill")
         pools = _kv4_ptrs(k_pool, v_pool) if kv4 else (k_pool.data_ptr(), v_pool.data_ptr())
         _lib.call(("fe_prefill_paged_kv4" if kv4 else "fe_prefill_paged_window") + _SFX[q.dtype],
                   q.data_ptr(), out.data_ptr(), *pools, nb, block_tables.data_ptr(),
                   block_tables.shape[1], q_offsets.data_ptr(), context_lens.data_ptr(), num_seqs,
-                  total_q, hq, hkv, d, bs, float(scale), window, sinks, _ptr(workspace),
-                  0 if workspace is None else workspace.numel() * workspace.element_size(),
-                  _stream(dev))
+                  total_q, hq, hkv, d, bs, float(scale), window, sinks, workspace.data_ptr(),
+                  workspace.numel() * workspace.element_size(), _stream(dev))
         return out
     need = int(_lib.load().fe_prefill_workspace_size(num_seqs, total_q, hq, hkv, d))
     ws = decode_workspace(dev, need, kind="prefill") if workspace is None else workspace

@@ -138,13 +138,13 @@ int fe_paged_decode_kv4_bf16(const void* q, int64_t q_batch_stride, void* out, c
                              int head_dim, int block_size, float scale, int window, int sinks,
                              int target_splits, fe_stream_t stream);
 
-/* Workspace bytes of the 16-bit and 4-bit prefill forms below (the decode's rules). */
+/* Workspace bytes of the prefill forms below (the decode's rules). */
 size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int num_q_heads, int kv_heads,
                                       int head_dim);
 
 /*
  * fe_prefill_paged (flexengine_amd.h) under a window with sinks: the same rows, tables and
- * offsets, scale > 0.  fp32 needs no workspace (null allowed).
+ * offsets, scale > 0.
  */
 int fe_prefill_paged_window(const void* q, void* out, const void* k_pool, const void* v_pool,
                             int num_blocks, const int32_t* block_tables, int table_stride,

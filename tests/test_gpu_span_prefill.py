@@ -211,3 +211,16 @@ def test_prefill_refusals_on_the_gpu():
         s.run(workspace=torch.zeros(256, dtype=torch.uint8, device=DEV))
     with pytest.raises(ValueError):
         ops.prefill_paged(s.q.bfloat16().to(DEV), s.kp, s.vp, s.tabs, s.offs, s.ctx, 20)
+
+
+@pytest.mark.parametrize("dt,bits,d", [(F32, 32, 96), (F32, 32, 128), (F16, 16, 72), (BF16, 4, 160), (F16, 16, 256)])
+def test_prefill_splits_at_other_head_dims(dt, bits, d):
+    s = Step([(4000, 9), (0, 2), (2990, 30)], 16, 6, 2, d, dt, bits, 2600, 20, 44)
+    got = s.run()
+    s.check(got, rows=12)
+    assert torch.equal(s.run(), got)
+
+
+def test_prefill_splits_of_many_kv_heads_fit_the_workspace():
+    s = Step([(1500, 1)], 16, 96, 96, 8, F32, 32, 1200, 0, 45)
+    s.check()

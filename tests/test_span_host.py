@@ -68,9 +68,8 @@ def test_attention_forms_refuse_on_the_host(lib, call, kind, sfx):
     for bs in (8, 24, 0):
         assert go(bs=bs) == UNSUPPORTED, bs
     assert go(nb=1 << 30) == UNSUPPORTED               # pool rows past 32 bits
-    if (call, sfx) != (prefill, "_f32"):               # (that one has no workspace)
-        assert go() == WORKSPACE and go(ws=None, ws_bytes=1 << 40) == WORKSPACE
-        assert go(ws=ctypes.c_void_p(260), ws_bytes=1 << 40) == WORKSPACE
+    assert go() == WORKSPACE and go(ws=None, ws_bytes=1 << 40) == WORKSPACE
+    assert go(ws=ctypes.c_void_p(260), ws_bytes=1 << 40) == WORKSPACE
 
 
 @pytest.mark.parametrize("kind,sfx", FORMS)
