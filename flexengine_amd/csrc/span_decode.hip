@@ -539,7 +539,7 @@ __device__ __forceinline__ void merge_pieces(const SpanArgs& a, int b, int h, in
     const int d = e4 * 4 - hh * D;  // the partials keep D's layout
     if (!PAD || d < a.dr)
       store_out4<E>(a.out, ((int64_t)b * a.Hq + h * G + hh) * (PAD ? a.dr : D) + d,
-                    num * (1.f / den));
+                    num * (den > 0.f ? 1.f / den : 0.f));
   }
 }
 

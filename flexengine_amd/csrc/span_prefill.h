@@ -7,15 +7,15 @@
 // Work split: for one KV head the rows of a sequence are the pairs (position, query head of the
 // group), position-major (row r: position r / G), so the G heads share what is read of K and V.
 // A unit is 32 * NW such rows of one sequence and KV head, one workgroup of NW waves of 32 rows
-// each; it walks the 64-key blocks from the first to the sinks' last and then from the one that
-// holds its first row's window start to its last row's position.  Blocks between are not read,
-// keys of an edge block that no row of the unit sees are taken as zeros (their pages may hold
+// each; it walks the 16-key tiles from the first to the sinks' last and then from the one that
+// holds its first row's window start to its last row's position, four at a time.  Tiles between
+// are not read, keys that no row of the unit sees are taken as zeros (their pages may hold
 // anything).  Where the units are too few for the chip, up to KS workgroups share one, each an
 // equal run of its blocks: each writes normalised fp32 rows and base-2 log-sum-exps with
 // device-coherent stores, waits for them and draws a ticket; the last one merges and sets the
 // ticket back to zero.
 //
-// One block (lane (hf, n) = (lane / 32, lane % 32) holds row n of its wave), both products on
+// One block of four tiles (lane (hf, n) = (lane / 32, lane % 32) holds row n of its wave), both products on
 // v_mfma_f32_32x32x16:
 //   S^T[32 keys x 32 rows] = K.Q^T, two key tiles; register i holds the score of key 8 (i / 4)
 //     + 4 hf + i % 4 of the tile, so a row's maximum takes one exchange between the halves;
@@ -27,9 +27,9 @@
 // banks busy in both reads), two stages: while one block is computed the next arrives.  16-bit
 // pools come by LDS DMA (buffer_load ... lds), one 8- or 16-key run a wave.  4-bit pools come
 // through registers: a thread loads 16-byte chunks -- 32 codes, one block with one scale --
-// two key blocks ahead, and converts them (16 conversions and four 16-byte LDS writes a chunk)
-// one block ahead; at D = 128 and NW = 8 that is one chunk a thread and block, beside the 48
-// matrix instructions of its wave.
+// two blocks ahead, and converts them (16 conversions and four 16-byte LDS writes a chunk) one
+// block ahead; at D = 128 and NW = 8 that is one chunk a thread and block, beside the 32 matrix
+// instructions of its wave.
 #pragma once
 
 #include "kv4.h"

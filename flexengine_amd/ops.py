@@ -382,7 +382,9 @@ def decode_workspace(device: torch.device, nbytes: int, kind: str = "decode") ->
     Calls on one stream are ordered, so sharing is safe there; callers running
     these kernels on several streams at once must pass their own zero-filled
     workspace.  A larger request replaces the buffer; see hold_workspaces() for
-    callers that record the kernels into a graph.
+    callers that record the kernels into a graph.  One that is first made while a
+    stream is captured is that call's alone: the graph's memory holds it and its
+    replays fill it with zeros, so no call outside the graph can use it.
     """
     key = (device.type, device.index, kind)
     ws = _WORKSPACES.get(key)
@@ -390,7 +392,8 @@ def decode_workspace(device: torch.device, nbytes: int, kind: str = "decode") ->
         # zero-filled once: the split-K tickets at its start must begin at zero
         # (every call leaves them at zero again)
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = ws
+        if not torch.cuda.is_current_stream_capturing():
+            _WORKSPACES[key] = ws
     for held in _HOLDERS:
         if not any(t is ws for t in held):
             held.append(ws)
@@ -502,6 +505,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no decode plan")
+        _require_gpu(q, workspace)
         if workspace is None:
             workspace = decode_workspace(dev, _pure_size(
                 "fe_span_decode_workspace_size", batch, hq, hkv, d, block_tables.shape[1] * bs,
@@ -719,6 +723,7 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no prefill plan")
+        _require_gpu(q, workspace)
         if workspace is None:
             workspace = decode_workspace(dev, int(_lib.load().fe_span_prefill_workspace_size(
                 num_seqs, total_q, hq, hkv, d)), kind="span_prefill")

@@ -5,7 +5,10 @@
  * Window.  A query at position p of its sequence sees the keys j <= p with p - j < window, and
  * the sequence's first `sinks` keys whatever the distance.  window 0: every key j <= p (the
  * 4-bit forms; the _window forms take window >= 1), sinks then has no effect.  Pages that no
- * query of the call sees, and their table entries, are not read and may hold anything.
+ * query of the call sees, and their table entries, are not read and may hold anything, as may
+ * keys of other pages that none sees.  The prefill forms compute up to 128 (fp32: 16; long 4-bit
+ * prompts: 256) rows of a sequence together: a V that is infinite or NaN and seen by one of them
+ * makes NaN of the others too (0 * inf).
  *
  * 4-bit pools.  A row of one token and KV head is cut into blocks of 32 dims: 32 e2m1 codes (0,
  * 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with one e8m0 scale byte s, values code *
@@ -16,12 +19,13 @@
  * A write takes the smallest power of two 2^e with max|x| <= 7 * 2^e, -23 <= e <= 13 (fp16
  * rows) or 125 (bf16 rows), and rounds to the nearest code, ties to the even one.  Every value
  * is exact in the rows' type.  fp16 magnitudes above 49152 are held as 49152; a block with an
- * infinity or a NaN is held as NaN.
+ * infinity or a NaN is held as NaN.  Two rows of one call in the same slot leave it undefined.
  *
  * Shapes: block_size a power of two, of at least 16 for attention; head_dim a multiple of 32 up
  * to 256 (4-bit), a multiple of 8 up to 256 (fp16, bf16 windows) or up to 128 (fp32 windows);
- * tables of up to 262144 tokens; any number of query heads per KV head (above 16 they are
- * attended in groups, each reading K and V).  No plans, and no shared-prefix form.
+ * tables of up to 262144 tokens (decode); any number of query heads per KV head (above 16 the
+ * decode attends them in groups, each reading K and V), batch * kv_heads * groups up to 65536
+ * there.  No plans, and no shared-prefix form.
  */
 #ifndef FLEXENGINE_AMD_SPAN_H
 #define FLEXENGINE_AMD_SPAN_H

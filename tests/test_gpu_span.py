@@ -316,6 +316,164 @@ def test_decode_on_two_streams_with_their_own_workspaces():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def high_rows(nb, bs, hkv, d, dt, bits, blocks, k, v):
+    """Pools of nb blocks, nothing but `blocks` filled: with the rows k, v [len(blocks) * bs, hkv, d]."""
+    slots = [t.repeat_interleave(bs) if i == 0 else t.repeat(len(blocks)) for i, t in enumerate(
+        (torch.tensor(blocks, dtype=torch.int32, device=DEV), torch.arange(bs, dtype=torch.int32, device=DEV)))]
+    if bits == 4:
+        make = lambda: ops.Kv4Pool(torch.empty(nb, hkv, bs, d // 2, dtype=torch.uint8, device=DEV),  # noqa: E731
+                                   torch.empty(nb, hkv, bs, d // 32, dtype=torch.uint8, device=DEV), dt)
+    else:
+        make = lambda: torch.empty(nb, bs, hkv, d, dtype=dt, device=DEV)  # noqa: E731
+    kp, vp = make(), make()
+    ops.write_kv(k.to(DEV), v.to(DEV), kp, vp, *slots)
+    return kp, vp
+
+
+@pytest.mark.parametrize("dt,bits,nb", [(F16, 16, 140000), (F32, 32, 70000), (BF16, 4, 300000)])
+def test_pools_past_32_bit_offsets(dt, bits, nb):
+    """The last blocks of pools whose elements (4-bit: bytes) pass 2^32 (fp32: 2^31): written in
+    every way, gathered, attended by a decode with a new row and by a prefill."""
+    bs, hkv, d, hq, n = 32, 8, 128, 16, 100
+    assert nb * bs * hkv * d >> (1 if bits == 4 else 0) >= 1 << (31 if bits == 32 else 32)
+    blocks = [nb - 1, nb - 5, nb // 2 + 7, nb - 2]
+    k = torch.randn(4 * bs, hkv, d, generator=gen(70)).to(dt)
+    v = torch.randn(4 * bs, hkv, d, generator=gen(71)).to(dt)
+    kp, vp = high_rows(nb, bs, hkv, d, dt, bits, blocks, k, v)
+    tabs = torch.tensor([blocks], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([n], dtype=torch.int32, device=DEV)
+    offs = torch.tensor([0, 40], dtype=torch.int32, device=DEV)
+    ops.write_kv_ragged(k[60:n].to(DEV), v[60:n].to(DEV), kp, vp, tabs, offs, ctx)
+    ops.write_kv_decode(k[n - 1:n].to(DEV), v[n - 1:n].to(DEV), kp, vp, tabs, ctx)
+    hold = R.round4 if bits == 4 else (lambda x: x.double())
+    ko, vo = ops.gather_kv(kp, vp, tabs, ctx, torch.tensor([0, n], dtype=torch.int32, device=DEV), n)
+    assert torch.equal(ko.double().cpu(), hold(k[:n])) and torch.equal(vo.double().cpu(), hold(v[:n]))
+    q = torch.randn(40, hq, d, generator=gen(72)).to(dt)
+    got = ops.prefill_paged(q.to(DEV), kp, vp, tabs, offs, ctx, 40, window=50, sinks=3)
+    R.assert_close(got, *R.attend(q, hold(k[:n]), hold(v[:n]), torch.arange(60, n), 50, 3))
+    k[n], v[n] = k[0].clone(), v[3].clone()
+    got = ops.paged_decode(q[:1].to(DEV), kp, vp, tabs, ctx + 1, k_new=k[n:n + 1].to(DEV),
+                           v_new=v[n:n + 1].to(DEV), window=70, sinks=5)
+    R.assert_close(got, *R.attend(q[:1], hold(k[:n + 1]), hold(v[:n + 1]), torch.tensor([n]), 70, 5))
+    ko, vo = ops.gather_kv(kp, vp, tabs, ctx + 1, torch.tensor([0, n + 1], dtype=torch.int32, device=DEV), n + 1)
+    assert torch.equal(ko.double().cpu(), hold(k[:n + 1])) and torch.equal(vo.double().cpu(), hold(v[:n + 1]))
+
+
+@pytest.mark.parametrize("s", [512, 513, 700])
+def test_ragged_writes_and_gathers_of_many_sequences(s):
+    r = random.Random(s)
+    lens = [r.randrange(0, 6) for _ in range(s)]
+    new = [r.randrange(0, n + 1) for n in lens]
+    tables, nb = paged(lens, 4, 1, s)
+    tabs, ctx = tables.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    offs = torch.tensor([sum(new[:i]) for i in range(s + 1)], dtype=torch.int32, device=DEV)
+    kp, vp = (ops.Kv4Pool.empty((nb, 4, 1, 32), F16) for _ in range(2))
+    k = torch.randn(sum(new), 1, 32, generator=gen(73)).half()
+    ops.write_kv_ragged(k.to(DEV), (-k).to(DEV), kp, vp, tabs, offs, ctx)
+    ends = torch.tensor([sum(lens[:i]) for i in range(s + 1)], dtype=torch.int32, device=DEV)
+    ko, vo = ops.gather_kv(kp, vp, tabs, ctx, ends, sum(lens))
+    want, at = [], 0
+    for n, m in zip(lens, new):
+        want += [torch.zeros(n - m, 1, 32, dtype=torch.float64), R.round4(k[at:at + m])]
+        at += m
+    want = torch.cat(want)
+    assert torch.equal(ko.double().cpu(), want) and torch.equal(vo.double().cpu(), -want)
+
+
+@pytest.mark.parametrize("dt,bits", [(F16, 4), (BF16, 16), (F32, 32)])
+@pytest.mark.parametrize("splits", [1, 16])
+def test_decode_non_finite_rows_are_nan_for_who_sees_them_alone(dt, bits, splits):
+    """A row's NaN or infinity reaches the queries of its sequence that see it, no others."""
+    n, window, sinks = 405, 64, 4
+    p = Pools([n, n, n, n], 16, 1, 64, dt, bits, 0, 0, 74)
+    want = Pools([n, n, n, n], 16, 1, 64, dt, bits, 0, 0, 74)
+    bad = torch.ones(1, 1, 64, dtype=dt, device=DEV)
+    bad[0, 0, 7] = math.nan
+
+    def put(b, j, pool_k):
+        rows = [torch.ones_like(bad), torch.ones_like(bad)]
+        rows[0 if pool_k else 1] = bad
+        blk = p.tabs[b, j // 16].reshape(1)
+        ops.write_kv(*rows, p.kp, p.vp, blk, torch.tensor([j % 16], dtype=torch.int32, device=DEV))
+
+    put(0, 350, True)        # seen: its K
+    put(1, 2, False)         # seen: a sink's V
+    put(2, 340, True)        # just before the window (341 on), in its first tile
+    put(2, 336, False)
+    put(3, 4, False)         # behind the sinks, in their tile
+    q = torch.randn(4, 8, 64, generator=gen(75)).to(dt).to(DEV)
+    run = lambda s: ops.paged_decode(q, s.kp, s.vp, s.tabs, s.ctx, window=window,  # noqa: E731
+                                     sinks=sinks, target_splits=splits)
+    got, ref = run(p), run(want)
+    assert torch.equal(got[2:], ref[2:]) and torch.isfinite(ref).all()
+    assert torch.isnan(got[0]).all()
+    seen = torch.isnan(got[1])   # of the row, or the 4-bit row's block
+    assert seen[:, 7].all() and seen[:, :32].all() == (bits == 4) and not seen[:, 32:].any()
+
+
+@pytest.mark.parametrize("dt,bits", [(F16, 4), (F16, 16), (F32, 32)])
+def test_decode_lengths_past_the_table_end_at_it(dt, bits):
+    p = Pools([64, 40], 16, 2, 64, dt, bits, 0, 0, 76)
+    width = 3                         # tables of 48 tokens
+    tabs = p.tabs[:, :width].contiguous()
+    q = torch.randn(2, 4, 64, generator=gen(77)).to(dt).to(DEV)
+    long = torch.tensor([1 << 30, 40], dtype=torch.int32, device=DEV)
+    cut = torch.tensor([48, 40], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.paged_decode(q, p.kp, p.vp, tabs, long, window=20, sinks=2),
+                       ops.paged_decode(q, p.kp, p.vp, tabs, cut, window=20, sinks=2))
+    neg = torch.tensor([-5, 40], dtype=torch.int32, device=DEV)
+    got = ops.paged_decode(q, p.kp, p.vp, tabs, neg, window=20, sinks=2)
+    assert (got[0] == 0).all() and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dt,bits", [(F16, 4), (F16, 16), (F32, 32)])
+def test_decode_new_rows_without_a_page_are_not_written(dt, bits):
+    p = Pools([33, 33], 16, 2, 64, dt, bits, 0, 0, 78)
+    tabs = p.tabs.clone()
+    tabs[0, 2] = JUNK                 # the new token's page
+    q = torch.randn(2, 4, 64, generator=gen(79)).to(dt).to(DEV)
+    kn = torch.randn(2, 2, 64, generator=gen(80)).to(dt).to(DEV)
+    raw = lambda: [t.clone() for x in (p.kp, p.vp) for t in ((x.codes, x.scales) if bits == 4 else (x,))]  # noqa: E731
+    before = raw()
+    blk = int(p.tabs[1, 2])
+    a = ops.paged_decode(q, p.kp, p.vp, tabs, p.ctx, k_new=kn, v_new=kn, window=30, sinks=2)
+    for x, y in zip(before, raw()):
+        same = (x.view(torch.uint8) == y.view(torch.uint8)).flatten(1).all(1)
+        same[blk] = True
+        assert same.all()
+    assert torch.isfinite(a[1]).all()
+
+
+@pytest.mark.parametrize("kind", ["decode", "prefill"])
+def test_a_workspace_made_in_a_capture_is_the_graphs_alone(kind):
+    p = Pools([3000], 16, 2, 128, F16, 4, 0, 0, 81)
+    q = torch.randn(1, 12, 128, generator=gen(82)).half().to(DEV)
+    offs = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+
+    def step():
+        if kind == "decode":
+            return ops.paged_decode(q, p.kp, p.vp, p.tabs, p.ctx, window=2500, sinks=4)
+        return ops.prefill_paged(q, p.kp, p.vp, p.tabs, offs, p.ctx, 1, window=2500, sinks=4)
+
+    key = ("cuda", 0, "span_" + kind)
+    step()
+    kept = ops._WORKSPACES.pop(key)
+    try:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with ops.hold_workspaces() as held, torch.cuda.graph(graph):
+            a, b = step(), step()
+        assert len(held) == 2 and key not in ops._WORKSPACES
+        for i in range(4):
+            q.copy_(torch.randn(1, 12, 128, generator=gen(90 + i)).half())
+            want = step()             # before the first replay too
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(a, want) and torch.equal(b, want) and torch.equal(step(), want)
+    finally:
+        ops._WORKSPACES[key] = kept
+
+
 def test_refusals_on_the_gpu():
     p = Pools([40], 16, 2, 64, F16, 4, 0, 0, 30)
     q = torch.zeros(1, 4, 64, dtype=F16, device=DEV)

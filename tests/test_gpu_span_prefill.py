@@ -224,3 +224,44 @@ def test_prefill_splits_at_other_head_dims(dt, bits, d):
 def test_prefill_splits_of_many_kv_heads_fit_the_workspace():
     s = Step([(1500, 1)], 16, 96, 96, 8, F32, 32, 1200, 0, 45)
     s.check()
+
+
+@pytest.mark.parametrize("dt,bits", TYPES)
+def test_prefill_non_finite_keys_reach_who_sees_them_alone(dt, bits):
+    """A NaN key reaches the rows that see it (V of a row that some row of a unit sees has to be
+    finite: K's is NaN here), in the same chunk and in no other sequence."""
+    chunks, window, sinks = [(100, 60), (100, 60)], 24, 4
+    a, b = (Step(chunks, 16, 4, 2, 64, dt, bits, window, sinks, 46) for _ in range(2))
+    bad = torch.ones(1, 2, 64, dtype=dt, device=DEV)
+    keep = torch.zeros_like(bad)
+    bad[..., 7] = math.nan
+    at = 120
+    ops.write_kv(bad, keep, a.kp, a.vp, a.tabs[0, at // 16].reshape(1),
+                 torch.tensor([at % 16], dtype=torch.int32, device=DEV))
+    ops.write_kv(keep, keep, b.kp, b.vp, b.tabs[0, at // 16].reshape(1),
+                 torch.tensor([at % 16], dtype=torch.int32, device=DEV))
+    got, want = a.run(), b.run()
+    sees = torch.tensor([100 + i >= at and 100 + i - at < window for i in range(60)])
+    assert torch.isnan(got[:60].cpu()[sees]).all()
+    idx = torch.nonzero(~sees)[:, 0]
+    R.assert_close(got[idx.to(DEV)], *R.attend(a.q[idx], a.k[0], a.v[0], 100 + idx, window, sinks))
+    assert torch.equal(got[60:], want[60:]) and torch.isfinite(want).all()
+
+
+def test_prefill_workspaces_elsewhere_are_refused():
+    s = Step([(10, 20)], 16, 4, 2, 64, F16, 4, 8, 1, 47)
+    with pytest.raises(ValueError):
+        s.run(workspace=torch.zeros(1 << 24, dtype=torch.uint8))
+    with pytest.raises(ValueError):
+        ops.paged_decode(s.q[:1].to(DEV), s.kp, s.vp, s.tabs, s.ctx, window=8,
+                         workspace=torch.zeros(1 << 24, dtype=torch.uint8))
+
+
+def test_prefill_sequences_longer_than_their_tables_or_contexts_stay_in_bounds():
+    """Offsets past total_q, contexts past the table and shorter than the chunk: rows of other
+    sequences are as they were."""
+    s = Step([(10, 20), (40, 8)], 16, 4, 2, 64, F16, 16, 8, 1, 48)
+    want = s.run()
+    offs = torch.tensor([0, 20, 400], dtype=torch.int32, device=DEV)
+    got = ops.prefill_paged(s.q.to(DEV), s.kp, s.vp, s.tabs, offs, s.ctx, 20, window=8, sinks=1)
+    assert torch.equal(got, want)
