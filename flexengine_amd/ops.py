@@ -39,7 +39,8 @@ class Kv4Pool:
     codes uint8 [num_blocks, kv_heads, block_size, head_dim / 2], scales uint8 [num_blocks,
     kv_heads, block_size, head_dim / 32], both with the same leading layer dim if the pool
     holds several; dtype: the type of its rows (float16 or bfloat16).  pool[layer] is one
-    layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it."""
+    layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it.
+    The tensors' shapes and strides stay as they are at the pool's first use, which checks them."""
     codes: torch.Tensor
     scales: torch.Tensor
     dtype: torch.dtype = FP16
@@ -71,6 +72,26 @@ class Kv4Pool:
     @property
     def ndim(self) -> int:
         return self.codes.ndim
+
+    @functools.cached_property
+    def _layout(self) -> tuple[int, int, int, int]:
+        """(num_blocks, block_size, kv_heads, head_dim) of one layer's pool, its tensors checked
+        (once: on every call that was 1 us of host time)."""
+        codes, scales = self.codes, self.scales
+        if codes.ndim != 4:
+            raise ValueError("4-bit pools must hold one layer of [num_blocks, kv_heads, block_size]")
+        if self.dtype not in DTYPES_16:
+            raise ValueError("4-bit pools must hold float16 or bfloat16 rows")
+        nb, hkv, bs, half = codes.shape
+        if half % 16 or scales.shape != (nb, hkv, bs, half // 16) or not (
+                codes.dtype is scales.dtype is torch.uint8):
+            raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
+                             "[..., head_dim / 32] (head_dim a multiple of 32)")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("K/V pools must be contiguous")
+        if scales.device != codes.device:
+            raise ValueError(f"all tensors must be on {codes.device}")
+        return nb, bs, hkv, 2 * half
 
     @functools.cached_property
     def _layers(self) -> list["Kv4Pool"]:
@@ -133,24 +154,10 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor,
 def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
     if not (isinstance(k_pool, Kv4Pool) and isinstance(v_pool, Kv4Pool)):
         raise ValueError("K and V pools must both be 4-bit pools, or both tensors")
-    kc, ks, vc, vs = k_pool.codes, k_pool.scales, v_pool.codes, v_pool.scales
-    shape = kc.shape
-    if len(shape) != 4 or vc.shape != shape:
-        raise ValueError("4-bit pools must both hold one layer of [num_blocks, kv_heads, block_size]")
-    nb, hkv, bs, half = shape
-    if k_pool.dtype not in DTYPES_16 or v_pool.dtype != k_pool.dtype:
-        raise ValueError("4-bit pools must hold float16 or bfloat16 rows (both the same)")
-    scales = (nb, hkv, bs, half // 16)
-    if half % 16 or ks.shape != scales or vs.shape != scales or not (
-            kc.dtype is ks.dtype is vc.dtype is vs.dtype is torch.uint8):
-        raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
-                         "[..., head_dim / 32] (head_dim a multiple of 32)")
-    if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
-        raise ValueError("K/V pools must be contiguous")
-    dev = kc.device
-    if ks.device != dev or vs.device != dev:
-        raise ValueError(f"all tensors must be on {dev}")
-    return nb, bs, hkv, 2 * half
+    layout = k_pool._layout
+    if v_pool._layout != layout or v_pool.dtype != k_pool.dtype:
+        raise ValueError("K and V pools must have the same shape and hold rows of the same type")
+    return layout
 
 
 def _is_kv4(k_pool, v_pool) -> bool:
