@@ -31,7 +31,6 @@ _SFX = {FP16: "", BF16: "_bf16", FP32: "_f32"}
 _MOVER_SFX = {FP16: "", BF16: "", FP32: "_f32"}
 
 
-@dataclass(frozen=True)
 class Kv4Pool:
     """A K or V pool held in 4 bits (include/flexengine_amd_span.h): the functions below that
     take pools take a pair of these in the place of two tensors.
@@ -40,10 +39,14 @@ class Kv4Pool:
     kv_heads, block_size, head_dim / 32], both with the same leading layer dim if the pool
     holds several; dtype: the type of its rows (float16 or bfloat16).  pool[layer] is one
     layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it.
-    The tensors' shapes and strides stay as they are at the pool's first use, which checks them."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    dtype: torch.dtype = FP16
+    The tensors and their shapes stay as they are at the pool's first use, which checks them."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = FP16):
+        self.codes = codes
+        self.scales = scales
+        self.dtype = dtype
+        self._checked: tuple[int, int, int, int] | None = None
+        self._layers: list["Kv4Pool"] | None = None
 
     @classmethod
     def empty(cls, shape, dtype: torch.dtype = FP16, device="cuda:0") -> "Kv4Pool":
@@ -56,6 +59,9 @@ class Kv4Pool:
             raise ValueError("4-bit pools hold float16 or bfloat16 rows")
         return cls(torch.zeros((*lead, hkv, bs, d // 2), dtype=torch.uint8, device=device),
                    torch.full((*lead, hkv, bs, d // 32), 127, dtype=torch.uint8, device=device), dtype)
+
+    def __repr__(self) -> str:
+        return f"Kv4Pool(shape={self.shape}, dtype={self.dtype}, device={self.device})"
 
     @property
     def device(self) -> torch.device:
@@ -73,32 +79,34 @@ class Kv4Pool:
     def ndim(self) -> int:
         return self.codes.ndim
 
-    @functools.cached_property
-    def _layout(self) -> tuple[int, int, int, int]:
+    def layout(self) -> tuple[int, int, int, int]:
         """(num_blocks, block_size, kv_heads, head_dim) of one layer's pool, its tensors checked
         (once: on every call that was 1 us of host time)."""
+        if self._checked is not None:
+            return self._checked
         codes, scales = self.codes, self.scales
-        if codes.ndim != 4:
+        shape = codes.shape
+        if len(shape) != 4:
             raise ValueError("4-bit pools must hold one layer of [num_blocks, kv_heads, block_size]")
         if self.dtype not in DTYPES_16:
             raise ValueError("4-bit pools must hold float16 or bfloat16 rows")
-        nb, hkv, bs, half = codes.shape
+        nb, hkv, bs, half = shape
         if half % 16 or scales.shape != (nb, hkv, bs, half // 16) or not (
                 codes.dtype is scales.dtype is torch.uint8):
             raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
                              "[..., head_dim / 32] (head_dim a multiple of 32)")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("K/V pools must be contiguous")
-        if scales.device != codes.device:
+        if scales.get_device() != codes.get_device():
             raise ValueError(f"all tensors must be on {codes.device}")
-        return nb, bs, hkv, 2 * half
-
-    @functools.cached_property
-    def _layers(self) -> list["Kv4Pool"]:
-        return [Kv4Pool(c, s, self.dtype) for c, s in zip(self.codes.unbind(0), self.scales.unbind(0))]
+        self._checked = nb, bs, hkv, 2 * half
+        return self._checked
 
     def __getitem__(self, layer: int) -> "Kv4Pool":
         """The pool of one layer (views of this one's tensors)."""
+        if self._layers is None:
+            self._layers = [Kv4Pool(c, s, self.dtype)
+                            for c, s in zip(self.codes.unbind(0), self.scales.unbind(0))]
         return self._layers[layer]
 
 
@@ -154,8 +162,8 @@ def _check_pool(k_pool: torch.Tensor, v_pool: torch.Tensor,
 def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
     if not (isinstance(k_pool, Kv4Pool) and isinstance(v_pool, Kv4Pool)):
         raise ValueError("K and V pools must both be 4-bit pools, or both tensors")
-    layout = k_pool._layout
-    if v_pool._layout != layout or v_pool.dtype != k_pool.dtype:
+    layout = k_pool.layout()
+    if v_pool.layout() != layout or v_pool.dtype != k_pool.dtype:
         raise ValueError("K and V pools must have the same shape and hold rows of the same type")
     return layout
 
