@@ -177,11 +177,21 @@ def _any_pool(k_pool, v_pool) -> tuple[int, int, int, int]:
         _check_pool(k_pool, v_pool, KV_DTYPES)
 
 
-def _mover(base: str, tail: str, k_pool, v_pool) -> tuple[str, tuple]:
+# entry points of the page movers by pool type (a pair: the 4-bit pools' forms)
+_MOVERS = {
+    base + tail: ({dt: f"fe_{base}{tail}{sfx}" for dt, sfx in _MOVER_SFX.items()},
+                  {dt: f"fe_{base}4{tail}{_SFX[dt]}" for dt in DTYPES_16})
+    for base, tail in (("write_kv", ""), ("write_kv", "_decode"), ("write_kv", "_ragged"),
+                       ("gather_kv", ""))
+}
+
+
+def _mover(name: str, k_pool, v_pool) -> tuple[str, tuple]:
     """A page mover's entry point for these pools, and the pools' pointers."""
+    plain, four = _MOVERS[name]
     if isinstance(k_pool, Kv4Pool):
-        return f"fe_{base}4{tail}{_SFX[k_pool.dtype]}", _kv4_ptrs(k_pool, v_pool)
-    return f"fe_{base}{tail}{_MOVER_SFX[k_pool.dtype]}", (k_pool.data_ptr(), v_pool.data_ptr())
+        return four[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
+    return plain[k_pool.dtype], (k_pool.data_ptr(), v_pool.data_ptr())
 
 
 def _kv4_ptrs(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple:
@@ -214,23 +224,29 @@ def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
 # KV page write / gather
 # ---------------------------------------------------------------------------------------
 
+def _new_rows(k_new, v_new, dtype, hkv, d, rows: str) -> tuple[int, int]:
+    """Checks of the rows that are written; returns their count and stride."""
+    shape, stride = k_new.shape, k_new.stride()
+    if v_new.shape != shape or len(shape) != 3 or shape[1] != hkv or shape[2] != d:
+        raise ValueError(f"K/V shapes must be [{rows}, kv_heads, head_dim]")
+    if k_new.dtype != dtype or v_new.dtype != dtype:
+        raise ValueError("wrong KV dtype")
+    if v_new.stride() != stride or stride[2] != 1 or stride[1] != d:
+        raise ValueError("new K/V rows must have contiguous heads and equal strides")
+    return shape[0], stride[0]
+
+
 def write_kv(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
              slot_block: torch.Tensor, slot_offset: torch.Tensor) -> None:
     """k_pool[slot_block[t], slot_offset[t]] = k_new[t] (and v); negative blocks are skipped."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, slot_block, slot_offset)
     nb, bs, hkv, d = _any_pool(k_pool, v_pool)
-    if k_new.shape != v_new.shape or k_new.ndim != 3 or tuple(k_new.shape[1:]) != (hkv, d):
-        raise ValueError("K/V shapes must be [tokens, kv_heads, head_dim]")
-    if k_new.dtype != k_pool.dtype or v_new.dtype != k_pool.dtype:
-        raise ValueError("wrong KV dtype")
-    if k_new.stride() != v_new.stride() or k_new.stride(2) != 1 or k_new.stride(1) != d:
-        raise ValueError("new K/V rows must have contiguous heads and equal strides")
-    t = k_new.shape[0]
+    t, stride = _new_rows(k_new, v_new, k_pool.dtype, hkv, d, "tokens")
     slot_block, slot_offset = _int32(slot_block, "slot_block"), _int32(slot_offset, "slot_offset")
     if slot_block.shape != (t,) or slot_offset.shape != (t,):
         raise ValueError("slot arrays must be [tokens]")
-    name, pools = _mover("write_kv", "", k_pool, v_pool)
-    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+    name, pools = _mover("write_kv", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), stride, *pools, nb,
               slot_block.data_ptr(), slot_offset.data_ptr(), t, hkv, d, bs, _stream(dev))
 
 
@@ -242,19 +258,14 @@ def write_kv_ragged(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     context_lens[s] tokens (the arrays prefill_paged takes; fe_write_kv_ragged)."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, block_tables, q_offsets, context_lens)
     nb, bs, hkv, d = _any_pool(k_pool, v_pool)
-    if k_new.shape != v_new.shape or k_new.ndim != 3 or tuple(k_new.shape[1:]) != (hkv, d):
-        raise ValueError("K/V shapes must be [tokens, kv_heads, head_dim]")
-    if k_new.dtype != k_pool.dtype or v_new.dtype != k_pool.dtype:
-        raise ValueError("wrong KV dtype")
-    if k_new.stride() != v_new.stride() or k_new.stride(2) != 1 or k_new.stride(1) != d:
-        raise ValueError("new K/V rows must have contiguous heads and equal strides")
+    tokens, stride = _new_rows(k_new, v_new, k_pool.dtype, hkv, d, "tokens")
     block_tables = _int32(block_tables, "block_tables")
     q_offsets, context_lens = _int32(q_offsets, "q_offsets"), _int32(context_lens, "context_lens")
     s = context_lens.shape[0]
     if block_tables.ndim != 2 or block_tables.shape[0] != s or q_offsets.shape != (s + 1,):
         raise ValueError("block_tables must be [S, W], q_offsets [S+1], context_lens [S]")
-    name, pools = _mover("write_kv", "_ragged", k_pool, v_pool)
-    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+    name, pools = _mover("write_kv_ragged", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), stride, *pools, nb,
               block_tables.data_ptr(), block_tables.shape[1], q_offsets.data_ptr(),
               context_lens.data_ptr(), s, k_new.shape[0], hkv, d, bs, _stream(dev))
 
@@ -315,19 +326,13 @@ def write_kv_decode(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     """Writes row b at position context_lens[b]-1 of sequence b; rows with length 0 are skipped."""
     dev = _require_gpu(k_new, v_new, k_pool, v_pool, block_tables, context_lens)
     nb, bs, hkv, d = _any_pool(k_pool, v_pool)
-    batch = k_new.shape[0]
-    if k_new.shape != v_new.shape or tuple(k_new.shape[1:]) != (hkv, d):
-        raise ValueError("K/V shapes must be [batch, kv_heads, head_dim]")
-    if k_new.dtype != k_pool.dtype or v_new.dtype != k_pool.dtype:
-        raise ValueError("wrong KV dtype")
-    if k_new.stride() != v_new.stride() or k_new.stride(2) != 1 or k_new.stride(1) != d:
-        raise ValueError("new K/V rows must have contiguous heads and equal strides")
+    batch, stride = _new_rows(k_new, v_new, k_pool.dtype, hkv, d, "batch")
     block_tables = _int32(block_tables, "block_tables")
     context_lens = _int32(context_lens, "context_lens")
     if block_tables.ndim != 2 or block_tables.shape[0] != batch or context_lens.shape != (batch,):
         raise ValueError("block_tables must be [batch, W] and context_lens [batch]")
-    name, pools = _mover("write_kv", "_decode", k_pool, v_pool)
-    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), *pools, nb,
+    name, pools = _mover("write_kv_decode", k_pool, v_pool)
+    _lib.call(name, k_new.data_ptr(), v_new.data_ptr(), stride, *pools, nb,
               block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(), batch, hkv,
               d, bs, _stream(dev))
 
@@ -346,7 +351,7 @@ def gather_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
         raise ValueError("block_tables [batch, W], context_lens [batch], out_offsets [batch+1]")
     k_out = torch.empty((total_tokens, hkv, d), dtype=k_pool.dtype, device=dev)
     v_out = torch.empty_like(k_out)
-    name, pools = _mover("gather_kv", "", k_pool, v_pool)
+    name, pools = _mover("gather_kv", k_pool, v_pool)
     _lib.call(name, *pools, nb, block_tables.data_ptr(), block_tables.shape[1],
               context_lens.data_ptr(), out_offsets.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
               batch, total_tokens, hkv, d, bs, _stream(dev))
@@ -407,7 +412,7 @@ def decode_workspace(device: torch.device, nbytes: int, kind: str = "decode") ->
         # zero-filled once: the split-K tickets at its start must begin at zero
         # (every call leaves them at zero again)
         ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        if not torch.cuda.is_current_stream_capturing():
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
             _WORKSPACES[key] = ws
     for held in _HOLDERS:
         if not any(t is ws for t in held):
