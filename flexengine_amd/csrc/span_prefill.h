@@ -41,9 +41,11 @@ namespace {
 constexpr int kSpanKeys = 64;      // keys per staged block
 // Workgroups that run at once (two of four waves on each of 256 CUs)
 constexpr int kSpanSlots = 512;
-// Key splits: units of fewer blocks than kSpanSplitFrom are not split (500 fresh tokens of 12/2
-// heads in two 26.6 us, whole 20.2), and a split has kSpanShare blocks at least (eight chunks of
-// 64 over up to 4000: 4 blocks 61.7 us, 6 44.0, 8 44.0; one of 16: 25.9, 25.8, 28.9).
+// Key splits: units of fewer blocks than kSpanSplitFrom are not split, and a split has kSpanShare
+// blocks at least.  12/2 heads of 128, from / share 6 / 3, 8 / 4, 10 / 6 and 12 / 6: eight chunks
+// of 64 over up to 4000 cached 52.4, 47.6, 37.6, 37.7 us; four of 400 over up to 500 29.7, 29.1,
+// 25.1, 25.5; four of 256-500 over up to 3000 44.0, 44.0, 44.1, 42.7; one of 50 over 2000 23.4,
+// 23.5, 25.1, 25.1.
 constexpr int kSpanSplitFrom = 12;
 constexpr int kSpanShare = 6;
 constexpr int kSpanMaxSplits = 16;
@@ -203,6 +205,26 @@ struct SplitRows {
   }
 };
 
+// Output rows (position * Hq + head) of a unit's rows, without integer divisions: row r0 + r is x
+// = r0 % G + r rows on from r0 - r0 % G, and x / G is exact by float: x < G + 256 is at least half
+// a row from the next multiple of G, 0.5 / G of a quotient below 256 / G + 1 (G <= 2^20).
+struct UnitRows {
+  uint32_t base;
+  int rem, step;
+  float inv;
+  __device__ __forceinline__ UnitRows(const SpanPrefill& a, const SpanUnit& u, int r0, int h) {
+    const int q = r0 / a.G;
+    rem = r0 - q * a.G;
+    base = (uint32_t)((u.q0 + q) * a.Hq + h * a.G);
+    step = a.Hq - a.G;
+    inv = 1.f / (float)a.G;
+  }
+  __device__ __forceinline__ uint32_t operator()(int r) const {
+    const int x = rem + r;
+    return base + (uint32_t)(x + (int)(((float)x + 0.5f) * inv) * step);
+  }
+};
+
 // Whether this workgroup is the unit's last: its rows are complete before its ticket is drawn,
 // and the last one sets the ticket back to zero.
 __device__ __forceinline__ bool last_split(int* ticket, int splits, int* last) {
@@ -219,12 +241,14 @@ __device__ __forceinline__ bool last_split(int* ticket, int splits, int* last) {
 
 // Joins the splits of a unit's rows 0 .. r_last (row_of: their output rows) by T threads: the
 // splits' weights of every row into LDS (weight [splits][ROWS]), then thread -> (row, 4 dims),
-// four splits of MR rows in one round trip.  Four chunks of 256-500 over up to 3000 cached: six
-// rows 46.2 us, four 47.1, two 49.0, eight, which spills, 47.9; four with every thread's own
-// weights 49.1.
-template <class E, int D, bool PAD, int ROWS, int T, int MR, class RowOf>
+// kJoin splits of MR rows in one round trip.  Four chunks of 256-500 over up to 3000 cached,
+// rows x splits: 8 x 2 42.8 us, 8 x 1 43.0, 8 x 3, which spills, 43.7, 16 x 1 44.1, 6 x 4 44.7,
+// 4 x 2 44.5; with every thread's own weights 48; the next trip's loads in flight over a trip
+// (4 x 2) 44.6.
+constexpr int kJoin = 2;
+template <class E, int D, bool PAD, int ROWS, int T, int MR>
 __device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRows& part, int splits,
-                                            float* weight, int r_last, RowOf row_of) {
+                                            float* weight, int r_last, const UnitRows& row_of) {
   if ((int)threadIdx.x < ROWS) {
     const uint32_t orow = row_of(min((int)threadIdx.x, r_last));
     float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
@@ -257,15 +281,15 @@ __device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRow
       orow[i] = row_of(min(row0 + i * RPP, r_last));
       num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int s0 = 0; s0 < splits; s0 += 4) {
-      f32x4 ov[MR][4];
+    for (int s0 = 0; s0 < splits; s0 += kJoin) {
+      f32x4 ov[MR][kJoin];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kJoin; ++k)
         if (s0 + k < splits)  // workgroup-uniform
 #pragma unroll
           for (int i = 0; i < MR; ++i) ov[i][k] = part.load(s0 + k, orow[i], d4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kJoin; ++k)
         if (s0 + k < splits)
 #pragma unroll
           for (int i = 0; i < MR; ++i)
@@ -696,11 +720,8 @@ void span_prefill_kernel(const SpanPrefill a) {
   }
   if (!last_split(a.tickets + item * a.Hkv + h, splits, &last)) return;
   static_assert(kSpanMaxSplits * ROWS * sizeof(float) <= sizeof(k0), "weights fit a stage");
-  join_splits<E, D, PAD, ROWS, NW * kWave, 6>(
-      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0,
-      [&](int i) __attribute__((always_inline)) {
-        return (uint32_t)((u.q0 + (r0 + i) / G) * a.Hq + h * G + (r0 + i) % G);
-      });
+  join_splits<E, D, PAD, ROWS, NW * kWave, 8>(
+      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0, UnitRows(a, u, r0, h));
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -785,7 +806,7 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   if (bs_log2 < 0 || bs % kTile != 0) return FE_ERR_UNSUPPORTED;
   if (d > 256 || d % (Q4 ? kQ4Block : 8) != 0) return FE_ERR_UNSUPPORTED;
   // key positions, pool rows and the offsets within a run of keys are 32-bit in the kernel
-  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) ||
+  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) || hq / hkv > (1 << 20) ||
       (int64_t)num_blocks * bs >= ((int64_t)1 << 31) || (int64_t)hkv * d >= ((int64_t)1 << 25) ||
       (int64_t)total_q * (hq / hkv) >= ((int64_t)1 << 30))
     return FE_ERR_UNSUPPORTED;

@@ -139,10 +139,7 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   int* const last = reinterpret_cast<int*>(smem + Lds::last);
   if (!last_split(a.tickets + item * a.Hkv + h, splits, last)) return;
   join_splits<F32, D, PAD, ROWS, kF32Waves * kWave, 2>(
-      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0,
-      [&](int r) __attribute__((always_inline)) {
-        return (uint32_t)((u.q0 + (r0 + r) / G) * a.Hq + h * G + (r0 + r) % G);
-      });
+      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0, UnitRows(a, u, r0, h));
 }
 
 template <int D, bool PAD>
@@ -163,7 +160,7 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
                table_stride > 0 && window > 0 && sinks >= 0 && hq % hkv == 0 && scale > 0.f);
   const int bs_log2 = span_log2(bs);
   if (bs_log2 < 0 || bs % kTile != 0 || d > 128 || d % 8 != 0) return FE_ERR_UNSUPPORTED;
-  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) ||
+  if ((int64_t)table_stride * bs >= ((int64_t)1 << 30) || hq / hkv > (1 << 20) ||
       (int64_t)num_blocks * bs >= ((int64_t)1 << 31) || (int64_t)hkv * d >= ((int64_t)1 << 25) ||
       (int64_t)total_q * (hq / hkv) >= ((int64_t)1 << 30))
     return FE_ERR_UNSUPPORTED;
