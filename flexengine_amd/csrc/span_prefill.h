@@ -205,23 +205,28 @@ struct SplitRows {
   }
 };
 
-// Output rows (position * Hq + head) of a unit's rows, without integer divisions: row r0 + r is x
-// = r0 % G + r rows on from r0 - r0 % G, and x / G is exact by float: x < G + 256 is at least half
-// a row from the next multiple of G, 0.5 / G of a quotient below 256 / G + 1 (G <= 2^20).
+// Positions and output rows (token * Hq + head) of a unit's rows, without integer divisions: row
+// r0 + r is x = r0 % G + r rows on from r0 - r0 % G, and x / G is exact by float: x < G + 256 is at
+// least half a row from the next multiple of G, 0.5 / G of a quotient below 256 / G + 1
+// (G <= 2^20).
 struct UnitRows {
-  uint32_t base;
-  int rem, step;
+  int64_t base;
+  int q, rem, step;
   float inv;
   __device__ __forceinline__ UnitRows(const SpanPrefill& a, const SpanUnit& u, int r0, int h) {
-    const int q = r0 / a.G;
+    q = r0 / a.G;
     rem = r0 - q * a.G;
-    base = (uint32_t)((u.q0 + q) * a.Hq + h * a.G);
+    base = (int64_t)(u.q0 + q) * a.Hq + h * a.G;
     step = a.Hq - a.G;
     inv = 1.f / (float)a.G;
   }
-  __device__ __forceinline__ uint32_t operator()(int r) const {
+  // token of row r0 + r within the sequence's new ones
+  __device__ __forceinline__ int token(int r) const {
+    return q + (int)(((float)(rem + r) + 0.5f) * inv);
+  }
+  __device__ __forceinline__ int64_t operator()(int r) const {
     const int x = rem + r;
-    return base + (uint32_t)(x + (int)(((float)x + 0.5f) * inv) * step);
+    return base + x + (int64_t)(int)(((float)x + 0.5f) * inv) * step;
   }
 };
 
@@ -250,7 +255,7 @@ template <class E, int D, bool PAD, int ROWS, int T, int MR>
 __device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRows& part, int splits,
                                             float* weight, int r_last, const UnitRows& row_of) {
   if ((int)threadIdx.x < ROWS) {
-    const uint32_t orow = row_of(min((int)threadIdx.x, r_last));
+    const int64_t orow = row_of(min((int)threadIdx.x, r_last));
     float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
 #pragma unroll
     for (int s = 0; s < kSpanMaxSplits; ++s) {
@@ -274,11 +279,11 @@ __device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRow
   const int DR = PAD ? a.dr : D;
   const int d4 = (int)(threadIdx.x % TPR) * 4;
   for (int row0 = (int)threadIdx.x / TPR; row0 <= r_last; row0 += MR * RPP) {
-    uint32_t orow[MR];
+    uint32_t orow[MR];  // (split rows are few: their partials are under 2 GiB)
     f32x4 num[MR];
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-      orow[i] = row_of(min(row0 + i * RPP, r_last));
+      orow[i] = (uint32_t)row_of(min(row0 + i * RPP, r_last));
       num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int s0 = 0; s0 < splits; s0 += kJoin) {
@@ -613,8 +618,9 @@ void span_prefill_kernel(const SpanPrefill a) {
   const int r0 = u.block * ROWS;
   const int r_last = min(r0 + ROWS, total_rows) - 1;
 
+  const UnitRows rows(a, u, r0, h);
   SpanWalk wk;
-  wk.init(a.span, cached + r0 / G, cached + r_last / G);
+  wk.init(a.span, cached + rows.q, cached + rows.token(r_last - r0));
   const int nb = wk.blocks();
   const int splits = span_splits(a, work, nb, kSpanSlots);
   if (ks >= splits) return;
@@ -623,21 +629,22 @@ void span_prefill_kernel(const SpanPrefill a) {
   const int wr0 = r0 + 32 * w;
   const bool has_rows = wr0 <= r_last;
   // positions of the wave's first and last row, and where their windows start
-  const int p_first = cached + min(wr0, r_last) / G, p_last = cached + min(wr0 + 31, r_last) / G;
+  const int p_first = cached + rows.token(min(wr0, r_last) - r0);
+  const int p_last = cached + rows.token(min(wr0 + 31, r_last) - r0);
   const int lo_first = window_start(a.span, p_first), lo_last = window_start(a.span, p_last);
   const int row = wr0 + n;
   const bool valid = row < total_rows;
   const int rc = valid ? row : r_last;
   const int32_t* trow = a.tables + (int64_t)u.s * a.W;
   SpanRows<D> r;
-  r.pos = cached + rc / G;
+  r.pos = cached + rows.token(rc - r0);
   r.lo = window_start(a.span, r.pos);
   r.m = kNegInf;
   r.l = 0.f;
 #pragma unroll
   for (int x = 0; x < D / 32; ++x) r.o[x] = f32x16{};
   {
-    const f16* qrow = a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR + 8 * hf;
+    const f16* qrow = a.q + rows(rc - r0) * DR + 8 * hf;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
       r.qv[c] = valid && (!PAD || 16 * c + 8 * hf < DR) ? ld16(qrow + 16 * c) : f16x8{};
@@ -694,7 +701,7 @@ void span_prefill_kernel(const SpanPrefill a) {
   const float inv = l > 0.f ? 1.f / l : 0.f;
   if (splits == 1) {
     if (!valid) return;
-    f16* orow = a.out + ((int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G) * DR + 4 * hf;
+    f16* orow = a.out + rows(row - r0) * DR + 4 * hf;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
@@ -708,7 +715,7 @@ void span_prefill_kernel(const SpanPrefill a) {
 
   const SplitRows part(a, D);
   if (valid) {
-    const int64_t orow = (int64_t)(u.q0 + row / G) * a.Hq + h * G + row % G;
+    const int64_t orow = rows(row - r0);
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
@@ -721,7 +728,7 @@ void span_prefill_kernel(const SpanPrefill a) {
   if (!last_split(a.tickets + item * a.Hkv + h, splits, &last)) return;
   static_assert(kSpanMaxSplits * ROWS * sizeof(float) <= sizeof(k0), "weights fit a stage");
   join_splits<E, D, PAD, ROWS, NW * kWave, 8>(
-      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0, UnitRows(a, u, r0, h));
+      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0, rows);
 }
 
 // ---- host -----------------------------------------------------------------------------------

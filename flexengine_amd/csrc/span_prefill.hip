@@ -77,21 +77,23 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   core.knew_row = nullptr;
   core.vnew_row = nullptr;
   core.new_pos = -1;
+  const UnitRows rows(a, u, r0, h);
   SpanWalk wk;
-  wk.init(a.span, cached + r0 / G, cached + r_last / G);
+  wk.init(a.span, cached + rows.q, cached + rows.token(r_last - r0));
   core.tok_end = wk.key_end;
   core.sinks = wk.sinks;
   core.wmin = wk.ws;
   core.span_head = wk.head;
   core.span_skip = wk.skip;
-  core.limit[0] = valid ? cached + rc / G + 1 : 0;
-  core.wlo[0] = window_start(a.span, cached + rc / G);
+  const int pos = cached + rows.token(rc - r0);
+  core.limit[0] = valid ? pos + 1 : 0;
+  core.wlo[0] = window_start(a.span, pos);
   const int nt = (wk.key_end + kTile - 1) / kTile - wk.skip;
   const int splits = span_splits(a, work, wk.blocks(), kF32Slots);
   if (ks >= splits) return;
   const int ntiles = core.begin((int)((int64_t)nt * ks / splits) + w, kF32Waves,
                                 (int)((int64_t)nt * (ks + 1) / splits));
-  const float* qrow = (const float*)a.q + ((int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G) * DR;
+  const float* qrow = (const float*)a.q + rows(rc - r0) * DR;
 #pragma unroll
   for (int c = 0; c < Core::NC; ++c) {
     core.qv[0][c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -119,7 +121,7 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
     den += sc[v] * park_l[v * kWave + lane];
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  const int64_t orow = (int64_t)(u.q0 + rc / G) * a.Hq + h * G + rc % G;
+  const int64_t orow = rows(rc - r0);
   const SplitRows part(a, D);
   for (int x = w; x < NX; x += kF32Waves) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -139,7 +141,7 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   int* const last = reinterpret_cast<int*>(smem + Lds::last);
   if (!last_split(a.tickets + item * a.Hkv + h, splits, last)) return;
   join_splits<F32, D, PAD, ROWS, kF32Waves * kWave, 2>(
-      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0, UnitRows(a, u, r0, h));
+      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0, rows);
 }
 
 template <int D, bool PAD>
