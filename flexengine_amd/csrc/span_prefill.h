@@ -74,7 +74,7 @@ struct SpanPrefill {
   float* part_o;    // [KS][total_q * Hq][D]
   float* part_lse;  // [KS][total_q * Hq]
   int* tickets;     // [units bound][Hkv], zero between calls
-  int W, S, total_q, Hq, Hkv, G, BS, bs_log2, NB, KS;
+  int W, S, total_q, Hq, Hkv, G, BS, bs_log2, NB, KS, units;
   int dr;            // the real head_dim (PAD: below D)
   float scale_log2;
   Span span;
@@ -166,7 +166,7 @@ __device__ __forceinline__ int span_splits(const SpanPrefill& a, const SpanWork&
   // to 4000 cached 71 us, as a whole one 78.5, as 1/2 72.8)
   const int slots = chip - (int)((int64_t)work.units * a.Hkv * 5 / 8);
   if (slots <= 0) return 1;
-  const int share = max((int)(((int64_t)work.blocks * a.Hkv + slots - 1) / slots), kSpanShare);
+  const int share = max((int)ceilf((float)work.blocks * (float)a.Hkv / (float)slots), kSpanShare);
   return min((nb + share - 1) / share, a.KS);
 }
 
@@ -599,10 +599,10 @@ void span_prefill_kernel(const SpanPrefill a) {
   __shared__ int last;
   // Workgroups in the order of their split, within it the later units, which see more keys,
   // first: those without work (a unit has as many splits as its keys are worth) come last
-  const int items = (int)gridDim.x / (a.Hkv * a.KS);
-  const int h = (int)blockIdx.x % a.Hkv;
-  const int ks = (int)blockIdx.x / a.Hkv / items;
-  const int item = items - 1 - (int)blockIdx.x / a.Hkv % items;
+  const int at = (int)blockIdx.x / a.Hkv;
+  const int h = (int)blockIdx.x - at * a.Hkv;
+  const int item = a.units - 1 - at;
+  const int ks = blockIdx.y;
   SpanUnit u;
   SpanWork work;
   if (!find_unit<ROWS>(a, item, u, work)) return;
@@ -624,7 +624,7 @@ void span_prefill_kernel(const SpanPrefill a) {
   const int nb = wk.blocks();
   const int splits = span_splits(a, work, nb, kSpanSlots);
   if (ks >= splits) return;
-  const int j0 = (int)((int64_t)nb * ks / splits), j1 = (int)((int64_t)nb * (ks + 1) / splits);
+  const int j0 = nb * ks / splits, j1 = nb * (ks + 1) / splits;  // (nb < 2^24)
 
   const int wr0 = r0 + 32 * w;
   const bool has_rows = wr0 <= r_last;
@@ -787,7 +787,7 @@ inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d, i
 
 template <int D, class E, bool Q4, bool PAD>
 int span_launch(const SpanPrefill& a, const SpanShape& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.units * a.Hkv * a.KS));
+  const dim3 grid((unsigned)(p.units * a.Hkv), (unsigned)a.KS);
   if constexpr (D == 128 && Q4 && !PAD) {
     if (p.waves == 8) {
       hipLaunchKernelGGL((span_prefill_kernel<D, E, Q4, PAD, 8>), grid, dim3(8 * kWave), 0, s, a);
@@ -823,7 +823,8 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
   const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d, window, Q4);
-  if (p.units * hkv * p.ks >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
+  // (a grid's threads are counted in 32 bits)
+  if (p.units * hkv >= ((int64_t)1 << 23)) return FE_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned(workspace))
     return FE_ERR_WORKSPACE;
   SpanPrefill a{};
@@ -849,6 +850,7 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   a.bs_log2 = bs_log2;
   a.NB = num_blocks;
   a.KS = p.ks;
+  a.units = (int)p.units;
   a.dr = d;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, window > 0 ? sinks : 0};

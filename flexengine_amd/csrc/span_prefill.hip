@@ -38,11 +38,11 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   constexpr int NX = Core::NX;
   extern __shared__ __align__(16) unsigned char smem[];
   const int DR = PAD ? a.dr : D;
-  const int h = blockIdx.x % a.Hkv;
   // by split, then the later units, which see more keys, first
-  const int items = (int)gridDim.x / (a.Hkv * a.KS);
-  const int ks = (int)blockIdx.x / a.Hkv / items;
-  const int item = items - 1 - (int)blockIdx.x / a.Hkv % items;
+  const int at = (int)blockIdx.x / a.Hkv;
+  const int h = (int)blockIdx.x - at * a.Hkv;
+  const int item = a.units - 1 - at;
+  const int ks = blockIdx.y;
   SpanUnit u;
   SpanWork work;
   if (!find_unit<ROWS>(a, item, u, work)) return;
@@ -91,8 +91,7 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
   const int nt = (wk.key_end + kTile - 1) / kTile - wk.skip;
   const int splits = span_splits(a, work, wk.blocks(), kF32Slots);
   if (ks >= splits) return;
-  const int ntiles = core.begin((int)((int64_t)nt * ks / splits) + w, kF32Waves,
-                                (int)((int64_t)nt * (ks + 1) / splits));
+  const int ntiles = core.begin(nt * ks / splits + w, kF32Waves, nt * (ks + 1) / splits);
   const float* qrow = (const float*)a.q + rows(rc - r0) * DR;
 #pragma unroll
   for (int c = 0; c < Core::NC; ++c) {
@@ -146,10 +145,9 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
 
 template <int D, bool PAD>
 int launch_f32(const SpanPrefill& a, hipStream_t s) {
-  const int64_t units = ((int64_t)a.total_q * a.G + kTile - 1) / kTile + a.S;
-  if (units * a.Hkv * a.KS >= ((int64_t)1 << 31)) return FE_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD>), dim3((unsigned)(units * a.Hkv * a.KS)),
-                     dim3(kF32Waves * kWave), SpanF32Lds<D>::bytes, s, a);
+  hipLaunchKernelGGL((span_prefill_f32_kernel<D, PAD>),
+                     dim3((unsigned)(a.units * a.Hkv), (unsigned)a.KS), dim3(kF32Waves * kWave),
+                     SpanF32Lds<D>::bytes, s, a);
   return FE_LAUNCH_STATUS();
 }
 
@@ -171,6 +169,8 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
   const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
   const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d, window, false, kTile, kF32Slots);
+  // (a grid's threads are counted in 32 bits)
+  if (p.units * hkv >= ((int64_t)1 << 23)) return FE_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned(workspace))
     return FE_ERR_WORKSPACE;
   SpanPrefill a{};
@@ -194,6 +194,7 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
   a.bs_log2 = bs_log2;
   a.NB = num_blocks;
   a.KS = p.ks;
+  a.units = (int)p.units;
   a.dr = d;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, sinks};
