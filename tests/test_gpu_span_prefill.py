@@ -265,3 +265,95 @@ def test_prefill_sequences_longer_than_their_tables_or_contexts_stay_in_bounds()
     offs = torch.tensor([0, 20, 400], dtype=torch.int32, device=DEV)
     got = ops.prefill_paged(s.q.to(DEV), s.kp, s.vp, s.tabs, offs, s.ctx, 20, window=8, sinks=1)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt,bits", [(F16, 4), (BF16, 16), (F32, 32)])
+@pytest.mark.parametrize("kind", ["decode", "prefill"])
+def test_captured_calls_follow_lengths_offsets_and_tables(kind, dt, bits):
+    """Replays of one graph after its lengths, offsets and tables changed in place, between eager
+    calls of the same."""
+    steps = [Step(chunks, 16, 12, 2, 64, dt, bits, 300, 4, 50 + i) for i, chunks in enumerate(
+        ([(900, 20), (0, 64), (333, 6)], [(0, 1), (1000, 49), (700, 40)], [(500, 88), (20, 1), (0, 1)]))]
+    width = max(s.tabs.shape[1] for s in steps)
+    blocks = max(s.kp.shape[0] for s in steps)
+    wide = [torch.full((3, width), JUNK, dtype=torch.int32, device=DEV) for _ in steps]
+    for t, s in zip(wide, steps):
+        t[:, :s.tabs.shape[1]] = s.tabs
+
+    def parts(pool):
+        return (pool.codes, pool.scales) if bits == 4 else (pool,)
+
+    def grown(pool):
+        x = [torch.zeros((blocks,) + t.shape[1:], dtype=t.dtype, device=DEV) for t in parts(pool)]
+        return ops.Kv4Pool(*x, dt) if bits == 4 else x[0]
+
+    kp, vp, tabs, ctx = grown(steps[0].kp), grown(steps[0].vp), wide[0].clone(), steps[0].ctx.clone()
+    offs, q = steps[0].offs.clone(), steps[0].q.to(DEV)
+    rows = q if kind == "prefill" else q[:3].contiguous()
+
+    def load(i):
+        for mine, theirs in ((kp, steps[i].kp), (vp, steps[i].vp)):
+            for a, b in zip(parts(mine), parts(theirs)):
+                a[:b.shape[0]].copy_(b)
+        tabs.copy_(wide[i]), ctx.copy_(steps[i].ctx), offs.copy_(steps[i].offs)
+        rows.copy_(steps[i].q[:rows.shape[0]])
+
+    def call():
+        if kind == "decode":
+            return ops.paged_decode(rows, kp, vp, tabs, ctx, window=300, sinks=4)
+        return ops.prefill_paged(rows, kp, vp, tabs, offs, ctx, 88, window=300, sinks=4)
+
+    with ops.hold_workspaces() as held:
+        load(0)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+    assert held
+    for i in (1, 2, 0, 1):
+        load(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, call())
+        if kind == "prefill":
+            steps[i].check(got, rows=8)
+
+
+@pytest.mark.parametrize("dt,bits,window,sinks", [(F16, 4, 0, 0), (BF16, 16, 300000, 70), (F32, 32, 100000, 33)])
+def test_contexts_of_hundreds_of_thousands_of_tokens(dt, bits, window, sinks):
+    """Long tables over a few pages in turn: a prefill of three rows and a decode at the longest
+    table that it takes."""
+    n, d, bs, nb = 400_003, 32, 16, 64
+    k = torch.randn(nb * bs, 1, d, generator=gen(60)).to(dt)
+    v = torch.randn(nb * bs, 1, d, generator=gen(61)).to(dt)
+    pools = []
+    for x in (k, v):
+        pages = x.view(nb, bs, 1, d)
+        if bits == 4:
+            c, s = packed(pages.transpose(1, 2))
+            pools.append(ops.Kv4Pool(c.contiguous().to(DEV), s.contiguous().to(DEV), dt))
+        else:
+            pools.append(pages.to(DEV))
+    if bits == 4:
+        k, v = R.round4(k), R.round4(v)
+    q = torch.randn(3, 2, d, generator=gen(62)).to(dt)
+    span = dict(window=window, sinks=sinks) if window else {}
+
+    def rows(m):
+        return (torch.arange(m) // bs % nb) * bs + torch.arange(m) % bs
+
+    tabs = (torch.arange(-(-n // bs), dtype=torch.int32) % nb)[None].to(DEV)
+    offs = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    got = ops.prefill_paged(q.to(DEV), *pools, tabs, offs, torch.tensor([n], dtype=torch.int32, device=DEV), 3, **span)
+    at = rows(n)
+    R.assert_close(got, *R.attend(q, k[at], v[at], torch.arange(n - 3, n), window, sinks))
+    m = 262_144
+    tabs = (torch.arange(m // bs, dtype=torch.int32) % nb)[None].to(DEV)
+    got = ops.paged_decode(q[:1].to(DEV), *pools, tabs, torch.tensor([m], dtype=torch.int32, device=DEV), **span)
+    at = rows(m)
+    R.assert_close(got, *R.attend(q[:1], k[at], v[at], torch.tensor([m - 1]), window, sinks))
+    with pytest.raises(_lib.FlexEngineAMDError):
+        longer = torch.zeros(1, m // bs + 1, dtype=torch.int32, device=DEV)
+        ops.paged_decode(q[:1].to(DEV), *pools, longer, torch.tensor([m], dtype=torch.int32, device=DEV), **span)
