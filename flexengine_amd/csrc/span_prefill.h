@@ -52,6 +52,7 @@ constexpr int kSpanMaxSplits = 16;
 typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSpanTickets = 65536;
 constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
+constexpr int64_t kSpanPartBytes = (int64_t)1 << 30;  // of all split states
 constexpr int kSpanSc1 = 16;       // buffer-instruction cache policy: sc1 (device-coherent)
 // Blocks of a walk over which the reference of the softmax follows every block's maximum in
 // either direction (the probabilities' rounding is then relative to the block's own largest);
@@ -71,8 +72,7 @@ struct SpanPrefill {
   const int32_t* tables;
   const int32_t* q_off;
   const int32_t* ctx;
-  float* part_o;    // [KS][total_q * Hq][D]
-  float* part_lse;  // [KS][total_q * Hq]
+  unsigned char* parts;  // [units][Hkv][KS] split states
   int* tickets;     // [units bound][Hkv], zero between calls
   int W, S, total_q, Hq, Hkv, G, BS, bs_log2, NB, KS, units;
   int dr;            // the real head_dim (PAD: below D)
@@ -155,6 +155,14 @@ __device__ __forceinline__ bool find_unit(const SpanPrefill& a, int item, SpanUn
   return found;
 }
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)addr);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(addr >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
+                                           (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
 // ---- key splits -----------------------------------------------------------------------------
 
 // Splits of a unit of nb key blocks
@@ -170,38 +178,68 @@ __device__ __forceinline__ int span_splits(const SpanPrefill& a, const SpanWork&
   return min((nb + share - 1) / share, a.KS);
 }
 
-// The splits' rows: normalised fp32 outputs [KS][total_q * Hq][D] and base-2 log-sum-exps,
-// device-coherent (the host keeps them under 2 GiB)
-struct SplitRows {
-  __amdgpu_buffer_rsrc_t ro, rl;
-  int64_t rows;  // of a split
-  int D;
-  __device__ __forceinline__ SplitRows(const SpanPrefill& a, int d) {
-    rows = (int64_t)a.total_q * a.Hq;
-    D = d;
-    ro = __builtin_amdgcn_make_buffer_rsrc(a.part_o, 0, (int)(a.KS * rows * D * 4), 0x00020000);
-    rl = __builtin_amdgcn_make_buffer_rsrc(a.part_lse, 0, (int)(a.KS * rows * 4), 0x00020000);
+// The splits' states of a unit, [KS] jobs of C chunks of 16 bytes and a base-2 log-sum-exp for
+// each of T threads: normalised fp32 outputs as the threads hold them, so that a wave's access is
+// one run of memory and nothing is rearranged.  Device-coherent.  Four chunks of 256-500 over up
+// to 3000 cached 37.5 us; as output rows, joined row by row with weights in LDS, 42.5.
+template <int C, int T>
+struct SplitParts {
+  static constexpr int kLse = C * T * 16;
+  static constexpr int kBytes = kLse + T * 4;
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ SplitParts(const SpanPrefill& a, int item, int h) {
+    r = span_rsrc(a.parts + (int64_t)(item * a.Hkv + h) * a.KS * kBytes, a.KS * kBytes);
   }
-  __device__ __forceinline__ uint32_t at(int s, int64_t row) const {
-    return (uint32_t)(s * rows + row);
+  __device__ __forceinline__ void store(int s, const f32x4 (&v)[C], float lse) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(span_u32x4, v[c]), r,
+                                             s * kBytes + (c * T + threadIdx.x) * 16, 0, kSpanSc1);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, lse), r,
+                                          s * kBytes + kLse + threadIdx.x * 4, 0, kSpanSc1);
   }
-  __device__ __forceinline__ void store(int s, int64_t row, int d0, f32x4 v) const {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(span_u32x4, v), ro,
-                                           (at(s, row) * D + d0) * (uint32_t)sizeof(float), 0,
-                                           kSpanSc1);
+  struct State {
+    f32x4 v[C];
+    float lse;
+  };
+  __device__ __forceinline__ void load(int s, State& x) const {
+    x.lse = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                          r, s * kBytes + kLse + threadIdx.x * 4, 0, kSpanSc1));
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      x.v[c] = __builtin_bit_cast(
+          f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                     r, s * kBytes + (c * T + threadIdx.x) * 16, 0, kSpanSc1));
   }
-  __device__ __forceinline__ f32x4 load(int s, int64_t row, int d0) const {
-    return __builtin_bit_cast(
-        f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                   ro, (at(s, row) * D + d0) * (uint32_t)sizeof(float), 0, kSpanSc1));
-  }
-  __device__ __forceinline__ void store_lse(int s, int64_t row, float v) const {
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rl,
-                                          at(s, row) * (uint32_t)sizeof(float), 0, kSpanSc1);
-  }
-  __device__ __forceinline__ float load_lse(int s, int64_t row) const {
-    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-                                         rl, at(s, row) * (uint32_t)sizeof(float), 0, kSpanSc1));
+  // The join of the splits' states in their order, the next one's loads in flight meanwhile (the
+  // last one's once more at the end: without a branch around the loads the wait for one state
+  // leaves the next one's running).
+  __device__ __forceinline__ void join(int splits, f32x4 (&num)[C]) const {
+    float M = kNegInf, den = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) num[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto add = [&](const State& x) __attribute__((always_inline)) {
+      const float m = fmaxf(M, x.lse);
+      const float alpha = M == kNegInf ? 0.f : exp2f(M - m);
+      const float w = x.lse == kNegInf ? 0.f : exp2f(x.lse - m);
+      den = den * alpha + w;
+#pragma unroll
+      for (int c = 0; c < C; ++c) num[c] = num[c] * alpha + w * x.v[c];
+      M = m;
+    };
+    State x, y;
+    load(0, x);
+    for (int s = 0;; s += 2) {  // workgroup-uniform
+      load(min(s + 1, splits - 1), y);
+      add(x);
+      if (s + 1 >= splits) break;
+      load(min(s + 2, splits - 1), x);
+      add(y);
+      if (s + 2 >= splits) break;
+    }
+    const float inv = den > 0.f ? 1.f / den : 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) num[c] *= inv;
   }
 };
 
@@ -244,69 +282,6 @@ __device__ __forceinline__ bool last_split(int* ticket, int splits, int* last) {
   return true;
 }
 
-// Joins the splits of a unit's rows 0 .. r_last (row_of: their output rows) by T threads: the
-// splits' weights of every row into LDS (weight [splits][ROWS]), then thread -> (row, 4 dims),
-// kJoin splits of MR rows in one round trip.  Four chunks of 256-500 over up to 3000 cached,
-// rows x splits: 8 x 2 42.8 us, 8 x 1 43.0, 8 x 3, which spills, 43.7, 16 x 1 44.1, 6 x 4 44.7,
-// 4 x 2 44.5; with every thread's own weights 48; the next trip's loads in flight over a trip
-// (4 x 2) 44.6.
-constexpr int kJoin = 2;
-template <class E, int D, bool PAD, int ROWS, int T, int MR>
-__device__ __forceinline__ void join_splits(const SpanPrefill& a, const SplitRows& part, int splits,
-                                            float* weight, int r_last, const UnitRows& row_of) {
-  if ((int)threadIdx.x < ROWS) {
-    const int64_t orow = row_of(min((int)threadIdx.x, r_last));
-    float lv[kSpanMaxSplits], M = kNegInf, den = 0.f;
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) {
-      lv[s] = kNegInf;
-      if (s < splits) lv[s] = part.load_lse(s, orow);
-    }
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) M = fmaxf(M, lv[s]);
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s) {
-      lv[s] = lv[s] == kNegInf ? 0.f : exp2f(lv[s] - M);
-      den += lv[s];
-    }
-    const float inv = den > 0.f ? 1.f / den : 0.f;
-#pragma unroll
-    for (int s = 0; s < kSpanMaxSplits; ++s)
-      if (s < splits) weight[s * ROWS + threadIdx.x] = lv[s] * inv;
-  }
-  __syncthreads();
-  constexpr int TPR = D / 4, RPP = T / TPR;  // threads a row, rows a pass
-  const int DR = PAD ? a.dr : D;
-  const int d4 = (int)(threadIdx.x % TPR) * 4;
-  for (int row0 = (int)threadIdx.x / TPR; row0 <= r_last; row0 += MR * RPP) {
-    uint32_t orow[MR];  // (split rows are few: their partials are under 2 GiB)
-    f32x4 num[MR];
-#pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      orow[i] = (uint32_t)row_of(min(row0 + i * RPP, r_last));
-      num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int s0 = 0; s0 < splits; s0 += kJoin) {
-      f32x4 ov[MR][kJoin];
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k)
-        if (s0 + k < splits)  // workgroup-uniform
-#pragma unroll
-          for (int i = 0; i < MR; ++i) ov[i][k] = part.load(s0 + k, orow[i], d4);
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k)
-        if (s0 + k < splits)
-#pragma unroll
-          for (int i = 0; i < MR; ++i)
-            num[i] += weight[(s0 + k) * ROWS + min(row0 + i * RPP, ROWS - 1)] * ov[i][k];
-    }
-#pragma unroll
-    for (int i = 0; i < MR; ++i)
-      if (row0 + i * RPP <= r_last && (!PAD || d4 < DR))
-        store_out4<E>(a.out, (int64_t)orow[i] * DR + d4, num[i]);
-  }
-}
-
 template <int D, bool Q4>
 struct SpanCfg {
   static constexpr int ROWB = D * 2;                // LDS bytes per staged key row
@@ -332,14 +307,6 @@ __device__ __forceinline__ float other_half(float x, int hf) {
 
 typedef __attribute__((address_space(3))) void span_lds_void;
 typedef __attribute__((address_space(3))) s16x4 span_lds_s16x4;
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t span_rsrc(const void* base, uint32_t bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)addr);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(addr >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0,
-                                           (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
 
 // The state of a wave's 32 rows
 template <int D>
@@ -699,36 +666,24 @@ void span_prefill_kernel(const SpanPrefill a) {
 
   const float l = r.l + other_half(r.l, hf);
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (splits == 1) {
-    if (!valid) return;
-    f16* orow = a.out + rows(row - r0) * DR + 4 * hf;
+  f32x4 o[D / 8];  // chunk 4 x + i: dims 32 x + 8 i + 4 hf .. +3
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x)
+  for (int x = 0; x < D / 32; ++x)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const f32x4 t = {r.o[x][4 * q4], r.o[x][4 * q4 + 1], r.o[x][4 * q4 + 2], r.o[x][4 * q4 + 3]};
-        if (!PAD || 32 * x + 8 * q4 + 4 * hf < DR)
-          *reinterpret_cast<f16x4*>(orow + 32 * x + 8 * q4) = to16x4<E>(t * inv);
-      }
-    return;
+    for (int i = 0; i < 4; ++i)
+      o[4 * x + i] =
+          f32x4{r.o[x][4 * i], r.o[x][4 * i + 1], r.o[x][4 * i + 2], r.o[x][4 * i + 3]} * inv;
+  if (splits > 1) {
+    const SplitParts<D / 8, NW * kWave> part(a, item, h);
+    if (valid) part.store(ks, o, l > 0.f ? r.m + log2f(l) : kNegInf);
+    if (!last_split(a.tickets + item * a.Hkv + h, splits, &last)) return;
+    if (has_rows) part.join(splits, o);
   }
-
-  const SplitRows part(a, D);
-  if (valid) {
-    const int64_t orow = rows(row - r0);
+  if (!valid) return;
+  f16* orow = a.out + rows(row - r0) * DR + 4 * hf;
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const f32x4 t = {r.o[x][4 * q4], r.o[x][4 * q4 + 1], r.o[x][4 * q4 + 2], r.o[x][4 * q4 + 3]};
-        part.store(ks, orow, 32 * x + 8 * q4 + 4 * hf, t * inv);
-      }
-    if (hf == 0) part.store_lse(ks, orow, l > 0.f ? r.m + log2f(l) : kNegInf);
-  }
-  if (!last_split(a.tickets + item * a.Hkv + h, splits, &last)) return;
-  static_assert(kSpanMaxSplits * ROWS * sizeof(float) <= sizeof(k0), "weights fit a stage");
-  join_splits<E, D, PAD, ROWS, NW * kWave, 8>(
-      a, part, splits, reinterpret_cast<float*>(k0), r_last - r0, rows);
+  for (int c = 0; c < D / 8; ++c)
+    if (!PAD || 8 * c + 4 * hf < DR) *reinterpret_cast<f16x4*>(orow + 8 * c) = to16x4<E>(o[c]);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -747,7 +702,7 @@ struct SpanShape {
   int waves;  // per workgroup
   int64_t units;
   int ks;
-  size_t o, lse, bytes;  // workspace
+  size_t bytes;  // workspace: tickets, split states
 };
 // Eight waves a workgroup halve what a row block converts, but leave one workgroup a CU, whose
 // start and end nothing hides: for long prompts over 4-bit pools that fill the chip either way.
@@ -776,12 +731,12 @@ inline SpanShape span_shape(int num_seqs, int total_q, int hq, int hkv, int d, i
   int64_t ks = wgs > 0 ? 2 * chip / wgs : 1;
   ks = ks < 1 ? 1 : (ks > kSpanMaxSplits ? kSpanMaxSplits : ks);
   if (p.waves != 4 || p.units * hkv > kSpanTickets) ks = 1;
-  const int64_t part_rows = (int64_t)total_q * hq;
-  while (ks > 1 && ks * part_rows * span_dim(d) * (int64_t)sizeof(float) >= ((int64_t)1 << 31)) --ks;
+  // a split's rows and its threads' log-sum-exps (SplitParts)
+  const int64_t job = (int64_t)unit_rows * span_dim(d) * (int64_t)sizeof(float) +
+                      4 * kWave * (int64_t)sizeof(float);
+  while (ks > 1 && ks * p.units * hkv * job > kSpanPartBytes) --ks;
   p.ks = (int)ks;
-  p.o = kSpanTicketBytes;
-  p.lse = p.o + (ks > 1 ? span_align((size_t)ks * part_rows * span_dim(d) * sizeof(float)) : 0);
-  p.bytes = p.lse + (ks > 1 ? span_align((size_t)ks * part_rows * sizeof(float)) : 0);
+  p.bytes = kSpanTicketBytes + (ks > 1 ? (size_t)(ks * p.units * hkv * job) : 0);
   return p;
 }
 
@@ -838,8 +793,7 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   a.q_off = q_off;
   a.ctx = ctx;
   a.tickets = (int*)workspace;
-  a.part_o = (float*)((char*)workspace + p.o);
-  a.part_lse = (float*)((char*)workspace + p.lse);
+  a.parts = (unsigned char*)workspace + kSpanTicketBytes;
   a.W = table_stride;
   a.S = num_seqs;
   a.total_q = total_q;

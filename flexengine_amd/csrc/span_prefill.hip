@@ -120,27 +120,32 @@ void span_prefill_f32_kernel(const SpanPrefill a) {
     den += sc[v] * park_l[v * kWave + lane];
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  const int64_t orow = rows(rc - r0);
-  const SplitRows part(a, D);
-  for (int x = w; x < NX; x += kF32Waves) {
+  constexpr int C = NX / kF32Waves;
+  f32x4 o[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int x = w + kF32Waves * i;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < kF32Waves; ++v)
       // tile x as the 16 dims from 16 x (a lane parked its 4 dims from f32_dim0)
       acc += sc[v] * park[(v * NX + (x & ~3) + g) * kWave + 16 * (x & 3) + n];
-    const int d0 = 16 * x + 4 * g;
-    if (!valid) continue;
-    if (splits > 1)
-      part.store(ks, orow, d0, acc * inv);
-    else if (!PAD || d0 < DR)
-      store_out4<F32>(a.out, orow * DR + d0, acc * inv);
+    o[i] = acc * inv;
   }
-  if (splits == 1) return;
-  if (valid && w == 0 && g == 0) part.store_lse(ks, orow, den > 0.f ? M + log2f(den) : kNegInf);
-  int* const last = reinterpret_cast<int*>(smem + Lds::last);
-  if (!last_split(a.tickets + item * a.Hkv + h, splits, last)) return;
-  join_splits<F32, D, PAD, ROWS, kF32Waves * kWave, 2>(
-      a, part, splits, reinterpret_cast<float*>(smem), r_last - r0, rows);
+  if (splits > 1) {
+    const SplitParts<C, kF32Waves * kWave> part(a, item, h);
+    if (valid) part.store(ks, o, den > 0.f ? M + log2f(den) : kNegInf);
+    int* const last = reinterpret_cast<int*>(smem + Lds::last);
+    if (!last_split(a.tickets + item * a.Hkv + h, splits, last)) return;
+    part.join(splits, o);
+  }
+  if (!valid) return;
+  const int64_t orow = rows(row - r0) * DR;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int d0 = 16 * (w + kF32Waves * i) + 4 * g;
+    if (!PAD || d0 < DR) store_out4<F32>(a.out, orow + d0, o[i]);
+  }
 }
 
 template <int D, bool PAD>
@@ -175,8 +180,7 @@ int span_prefill_f32(const void* q, void* out, const void* k_pool, const void* v
     return FE_ERR_WORKSPACE;
   SpanPrefill a{};
   a.tickets = (int*)workspace;
-  a.part_o = (float*)((char*)workspace + p.o);
-  a.part_lse = (float*)((char*)workspace + p.lse);
+  a.parts = (unsigned char*)workspace + kSpanTicketBytes;
   a.q = (const f16*)q;
   a.out = (f16*)out;
   a.k_pool = k_pool;
