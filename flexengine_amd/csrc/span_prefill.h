@@ -41,13 +41,14 @@ namespace {
 constexpr int kSpanKeys = 64;      // keys per staged block
 // Workgroups that run at once (two of four waves on each of 256 CUs)
 constexpr int kSpanSlots = 512;
-// Key splits: units of fewer blocks than kSpanSplitFrom are not split, and a split has kSpanShare
-// blocks at least.  12/2 heads of 128, from / share 6 / 3, 8 / 4, 10 / 6 and 12 / 6: eight chunks
-// of 64 over up to 4000 cached 52.4, 47.6, 37.6, 37.7 us; four of 400 over up to 500 29.7, 29.1,
-// 25.1, 25.5; four of 256-500 over up to 3000 44.0, 44.0, 44.1, 42.7; one of 50 over 2000 23.4,
-// 23.5, 25.1, 25.1.
-constexpr int kSpanSplitFrom = 12;
+// Key splits have at least kSpanShare blocks, fewer down to kSpanShareLow where that leaves no
+// more than half the workgroups that run at once (two on a CU take nearly twice as long each), and
+// a unit is split into two such at least.  12/2 heads of 128 in 4 bits, six blocks at least / fewer
+// by that rule / four always: 500 fresh tokens 19.2, 17.9, 17.8 us; 500 over 600 cached 21.8, 18.9,
+// 18.8; 50 over 2000 21.6, 20.4, 20.3; 16 over 4000 22.0, 22.6, 22.4; four chunks of 400 over up to
+// 500 25.2, 25.3, 25.9; eight of 64 over up to 4000 33.5, 33.7, 42.1 (eight blocks at least: 34.1).
 constexpr int kSpanShare = 6;
+constexpr int kSpanShareLow = 4;
 constexpr int kSpanMaxSplits = 16;
 typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSpanTickets = 65536;
@@ -168,14 +169,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t span_rsrc(const void* base, ui
 // Splits of a unit of nb key blocks
 __device__ __forceinline__ int span_splits(const SpanPrefill& a, const SpanWork& work, int nb,
                                            int chip) {
-  if (a.KS == 1 || nb < kSpanSplitFrom) return 1;
+  if (a.KS == 1 || nb < 2 * kSpanShareLow) return 1;
   // equal shares of the work, so that all splits fit the chip at once: the units' last ones are
   // short, half a workgroup more a unit on average (counted as 5/8: two chunks of 1000 over up
   // to 4000 cached 71 us, as a whole one 78.5, as 1/2 72.8)
-  const int slots = chip - (int)((int64_t)work.units * a.Hkv * 5 / 8);
-  if (slots <= 0) return 1;
-  const int share = max((int)ceilf((float)work.blocks * (float)a.Hkv / (float)slots), kSpanShare);
-  return min((nb + share - 1) / share, a.KS);
+  const int ends = (int)((int64_t)work.units * a.Hkv * 5 / 8);
+  if (chip <= ends) return 1;
+  const float all = (float)work.blocks * (float)a.Hkv;
+  const int share = (int)ceilf(all / (float)(chip - ends));
+  const int spread = chip / 2 > ends ? (int)fminf(ceilf(all / (float)(chip / 2 - ends)), kSpanShare)
+                                     : kSpanShare;
+  const int least = max(spread, kSpanShareLow);
+  if (nb < 2 * least) return 1;
+  const int blocks = max(share, least);
+  return min((nb + blocks - 1) / blocks, a.KS);
 }
 
 // The splits' states of a unit, [KS] jobs of C chunks of 16 bytes and a base-2 log-sum-exp for
