@@ -12,10 +12,11 @@ namespace {
 // states are joined in LDS.  Bound by the fp32 MFMAs (154 TFLOP/s in a large product): three
 // chunks of 100-700 tokens of 12/2 heads under a window of 512 40.9 us, 65 TFLOP/s, half the
 // chip in its second round.  32 rows a workgroup, which halve the reads of K and V: 49.1 us,
-// and four chunks of 500 under 1024 120 -> 145; eight waves 50.5.  Units too few for the chip
-// share their keys out over splits, as the 16-bit kernel's do (span_prefill.h): 50 tokens over up
-// to 3000 under a window of 2000 38.3 -> 18.6 us, four chunks of 10-20 over up to 8000 under 4000
-// 92.6 -> 37.3 (four chunks of 500 at head_dim 96, not split, 128.5 -> 133 for its registers).
+// and four chunks of 500 under 1024 120 -> 145 (as two waves a 16-row tile 49.8 and 118.5);
+// eight waves 50.5.  Units too few for the chip share their keys out over splits, as the 16-bit
+// kernel's do (span_prefill.h): 50 tokens over up to 3000 under a window of 2000 38.3 -> 15.7 us,
+// four chunks of 10-20 over up to 8000 under 4000 92.6 -> 35.8 (four chunks of 500 at head_dim 96,
+// not split, 128.5 -> 132 for its registers).
 constexpr int kF32Waves = 4;
 constexpr int kF32Slots = 768;  // workgroups that run at once: three on each of 256 CUs
 
