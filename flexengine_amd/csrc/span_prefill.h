@@ -11,12 +11,12 @@
 // holds its first row's window start to its last row's position, four at a time.  Tiles between
 // are not read, keys that no row of the unit sees are taken as zeros (their pages may hold
 // anything).  Where the units are too few for the chip, up to KS workgroups share one, each an
-// equal run of its blocks: each writes normalised fp32 rows and base-2 log-sum-exps with
-// device-coherent stores, waits for them and draws a ticket; the last one merges and sets the
+// equal run of its blocks: each writes its normalised fp32 state and base-2 log-sum-exps with
+// device-coherent stores, waits for them and draws a ticket; the last one joins them and sets the
 // ticket back to zero.
 //
-// One block of four tiles (lane (hf, n) = (lane / 32, lane % 32) holds row n of its wave), both products on
-// v_mfma_f32_32x32x16:
+// One block of four tiles (lane (hf, n) = (lane / 32, lane % 32) holds row n of its wave), both
+// products on v_mfma_f32_32x32x16:
 //   S^T[32 keys x 32 rows] = K.Q^T, two key tiles; register i holds the score of key 8 (i / 4)
 //     + 4 hf + i % 4 of the tile, so a row's maximum takes one exchange between the halves;
 //   base-2 online softmax with the lazy rescale, masks only on blocks at an edge of some row;
@@ -53,7 +53,7 @@ constexpr int kSpanMaxSplits = 16;
 typedef uint32_t span_u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSpanTickets = 65536;
 constexpr size_t kSpanTicketBytes = kSpanTickets * sizeof(int);
-constexpr int64_t kSpanPartBytes = (int64_t)1 << 30;  // of all split states
+constexpr int64_t kSpanPartBytes = (int64_t)1 << 28;  // of all split states: fewer splits past it
 constexpr int kSpanSc1 = 16;       // buffer-instruction cache policy: sc1 (device-coherent)
 // Blocks of a walk over which the reference of the softmax follows every block's maximum in
 // either direction (the probabilities' rounding is then relative to the block's own largest);

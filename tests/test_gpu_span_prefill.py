@@ -357,3 +357,24 @@ def test_contexts_of_hundreds_of_thousands_of_tokens(dt, bits, window, sinks):
     with pytest.raises(_lib.FlexEngineAMDError):
         longer = torch.zeros(1, m // bs + 1, dtype=torch.int32, device=DEV)
         ops.paged_decode(q[:1].to(DEV), *pools, longer, torch.tensor([m], dtype=torch.int32, device=DEV), **span)
+
+
+@pytest.mark.parametrize("dt,bits", [(F16, 4), (F32, 32)])
+def test_one_row_chunks_of_many_sequences_over_long_contexts(dt, bits):
+    r = random.Random(7)
+    s = Step([(r.randrange(800, 1500), 1) for _ in range(150)], 16, 4, 1, 64, dt, bits, 1300, 20, 51)
+    got = s.run()
+    s.check(got)
+    assert torch.equal(s.run(), got)
+
+
+@pytest.mark.parametrize("dt,bits", TYPES)
+def test_non_finite_keys_in_a_split(dt, bits):
+    """A NaN in a split's keys makes NaN of the rows that see it once the splits are joined."""
+    s = Step([(3000, 4), (2900, 2)], 16, 4, 1, 64, dt, bits, 2500, 8, 52)
+    want = s.run()
+    bad = torch.full((1, 1, 64), math.nan, dtype=dt, device=DEV)
+    ops.write_kv(bad, bad, s.kp, s.vp, s.tabs[0, 1600 // 16].reshape(1),
+                 torch.zeros(1, dtype=torch.int32, device=DEV))
+    got = s.run()
+    assert torch.isnan(got[:4]).all() and torch.equal(got[4:], want[4:]) and torch.isfinite(want).all()

@@ -195,3 +195,13 @@ def test_ticket_protocol_of_the_new_kernels():
             for family in families:
                 assert any(family in k for k in found), f"{family} has no ticket in {name}"
             assert not bad, "\n".join(f"{n}: {r}" for n, r in bad)
+
+
+def test_the_prefill_workspace_stays_small_for_many_sequences(lib):
+    tickets = 65536 * 4
+    for seqs, total, hq, hkv, d in ((4, 1500, 12, 2, 128), (1000, 1000, 12, 2, 128), (64, 1280, 32, 8, 256),
+                                    (1, 1, 96, 96, 8), (1, 100000, 32, 8, 128), (5000, 5000, 8, 8, 64)):
+        need = lib.fe_span_prefill_workspace_size(seqs, total, hq, hkv, d)
+        assert tickets <= need <= tickets + (1 << 28), (seqs, total, need)
+    assert lib.fe_span_prefill_workspace_size(1, 100000, 32, 8, 128) == tickets   # fills the chip unsplit
+    assert lib.fe_span_prefill_workspace_size(4, 1500, 12, 2, 128) > tickets
