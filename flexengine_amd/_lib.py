@@ -112,6 +112,12 @@ SIGNATURES |= {
     "fe_prefill_paged_kv4": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i,
                                   _i, _f, _i, _i, _p, _sz, _p]),
 }
+# the forms with fe_kv4_strides: after the scales of V
+for _name, _at in (("fe_write_kv4", 7), ("fe_write_kv4_decode", 7), ("fe_write_kv4_ragged", 7),
+                   ("fe_gather_kv4", 4), ("fe_paged_decode_kv4", 10), ("fe_prefill_paged_kv4", 6)):
+    _ret, _args = SIGNATURES[_name]
+    SIGNATURES[_name + "_strided"] = SIGNATURES[_name + "_strided_bf16"] = (
+        _ret, _args[:_at] + [_p] + _args[_at:])
 for _name in ("fe_write_kv4", "fe_write_kv4_decode", "fe_write_kv4_ragged", "fe_gather_kv4",
               "fe_paged_decode_window", "fe_paged_decode_kv4", "fe_prefill_paged_window",
               "fe_prefill_paged_kv4"):

@@ -21,9 +21,11 @@
 // byte's low half), scales [num_blocks, kv_heads, block_size, head_dim / 32].  The head stands
 // before the token, unlike in the 16-bit pools: a 4-bit row is 64 bytes at head_dim 128, half
 // a cache line, and heads run on different XCDs, whose L2s would each fetch the whole line.
+// The _strided forms take the same dims in any order and with gaps (Q4Layout).
 #pragma once
 
 #include "attn_core.h"
+#include "flexengine_amd_span.h"
 
 namespace fe {
 
@@ -32,6 +34,69 @@ constexpr uint32_t kQ4ScaleLow = 127 - 23;
 template <class E>
 constexpr uint32_t kQ4ScaleHigh = __is_same(E, Bf16) ? 127 + 125 : 127 + 13;
 constexpr uint32_t kQ4ScaleNan = 255;
+
+// ---- where the rows are -------------------------------------------------------------------
+// Distances between blocks, heads and tokens, of the codes in units of 16 bytes (a block of 32
+// dims), of the scales in bytes.  A page and a position in it are 32-bit, what they are
+// multiplied by too: one multiply-add each into a 64-bit offset.
+struct Q4Layout {
+  uint32_t code_block, code_token, scale_block, scale_token;
+  int64_t code_head, scale_head;
+  // byte offsets of a row of head 0
+  __device__ __forceinline__ uint64_t code_row(int blk, int off) const {
+    return ((uint64_t)(uint32_t)blk * code_block + (uint64_t)(uint32_t)off * code_token) * 16;
+  }
+  __device__ __forceinline__ uint64_t scale_row(int blk, int off) const {
+    return (uint64_t)(uint32_t)blk * scale_block + (uint64_t)(uint32_t)off * scale_token;
+  }
+  __device__ __forceinline__ int64_t code_offset(int h) const { return h * code_head * 16; }
+  __device__ __forceinline__ int64_t scale_offset(int h) const { return h * scale_head; }
+};
+
+// Whether rows of `row` bytes at these strides (blocks, heads, tokens; those of a size of 1
+// count for nothing) lie apart from each other: each stride past all that the smaller ones span
+inline bool q4_rows_apart(const int64_t (&stride)[3], const int64_t (&size)[3], int64_t row) {
+  int order[3] = {0, 1, 2};
+  for (int i = 0; i < 2; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (stride[order[j]] < stride[order[i]]) {
+        const int t = order[i];
+        order[i] = order[j];
+        order[j] = t;
+      }
+  int64_t extent = row;
+  for (int i = 0; i < 3; ++i) {
+    const int k = order[i];
+    if (size[k] == 1) continue;
+    int64_t span;
+    if (stride[k] < extent || __builtin_mul_overflow(stride[k], size[k] - 1, &span) ||
+        __builtin_add_overflow(extent, span, &extent))
+      return false;
+  }
+  return true;
+}
+
+// The layout of pools of these sizes: the dense one, or what `s` says
+inline int q4_layout(const fe_kv4_strides* s, int nb, int hkv, int d, int bs, Q4Layout& l) {
+  const int64_t size[3] = {nb, hkv, bs};
+  const int64_t sb = d / kQ4Block;
+  int64_t g[3] = {size[1] * size[2] * sb, size[2] * sb, sb}, c[3] = {g[0] * 16, g[1] * 16, sb * 16};
+  if (s != nullptr)
+    for (int i = 0; i < 3; ++i) {
+      c[i] = s->codes[i];
+      g[i] = s->scales[i];
+    }
+  for (int i = 0; i < 3; ++i) {
+    if (size[i] == 1) c[i] = g[i] = 0;
+    FE_CHECK_ARG(c[i] >= 0 && g[i] >= 0 && c[i] % 16 == 0);
+  }
+  FE_CHECK_ARG(q4_rows_apart(c, size, sb * 16) && q4_rows_apart(g, size, sb));
+  // block strides are 32-bit units, and 16 tokens of a tile are within a 32-bit offset
+  if (c[0] >> 36 || g[0] >> 32 || c[2] >> 26 || g[2] >> 26) return FE_ERR_UNSUPPORTED;
+  l = Q4Layout{(uint32_t)(c[0] / 16), (uint32_t)(c[2] / 16), (uint32_t)g[0], (uint32_t)g[2],
+               c[1] / 16, g[1]};
+  return FE_OK;
+}
 
 template <class E>
 __device__ __forceinline__ float from16(f16 x) {

@@ -20,6 +20,7 @@ struct Q4Pools {
   uint8_t* k_scales;
   uint8_t* v_codes;
   uint8_t* v_scales;
+  Q4Layout rows;
 };
 
 constexpr int kThreads = 256;
@@ -138,6 +139,14 @@ struct Chunk {
   __device__ __forceinline__ uint32_t of_token(uint32_t cpr) const { return h * cpr + c; }
 };
 
+// byte offsets of a chunk's codes and of its block's scale
+__device__ __forceinline__ int64_t code_at(const Q4Layout& l, const Slot& s, const Chunk& ch) {
+  return (int64_t)l.code_row(s.block, s.offset) + l.code_offset(ch.h) + ch.c * 4;
+}
+__device__ __forceinline__ int64_t scale_at(const Q4Layout& l, const Slot& s, const Chunk& ch) {
+  return (int64_t)l.scale_row(s.block, s.offset) + l.scale_offset(ch.h) + (ch.c >> 2);
+}
+
 template <class E, class Slots>
 __global__ __launch_bounds__(kThreads) void write_kv4_kernel(const f16* __restrict__ k_new,
                                                              const f16* __restrict__ v_new,
@@ -166,14 +175,14 @@ __global__ __launch_bounds__(kThreads) void write_kv4_kernel(const f16* __restri
     if (!ch.on) continue;
     const Slot sl = at[ch.t];
     if (sl.block < 0) continue;
-    const int64_t row = ((int64_t)sl.block * Hkv + ch.h) * BS + sl.offset;
     uint32_t ks, vs;
     const uint32_t kc = q4_quad<E>(k, ks), vc = q4_quad<E>(v, vs);
-    *reinterpret_cast<uint32_t*>(p.k_codes + row * (D / 2) + ch.c * 4) = kc;
-    *reinterpret_cast<uint32_t*>(p.v_codes + row * (D / 2) + ch.c * 4) = vc;
+    const int64_t co = code_at(p.rows, sl, ch), so = scale_at(p.rows, sl, ch);
+    *reinterpret_cast<uint32_t*>(p.k_codes + co) = kc;
+    *reinterpret_cast<uint32_t*>(p.v_codes + co) = vc;
     if ((ch.c & 3) == 0) {
-      p.k_scales[row * (D / kQ4Block) + (ch.c >> 2)] = (uint8_t)ks;
-      p.v_scales[row * (D / kQ4Block) + (ch.c >> 2)] = (uint8_t)vs;
+      p.k_scales[so] = (uint8_t)ks;
+      p.v_scales[so] = (uint8_t)vs;
     }
   }
 }
@@ -207,11 +216,11 @@ __global__ __launch_bounds__(kThreads) void gather_kv4_kernel(
     const Chunk ch(i, n, total, cpr);
     const Slot sl = at[ch.t];
     if (sl.block < 0) continue;
-    const int64_t row = ((int64_t)sl.block * Hkv + ch.h) * BS + sl.offset;
-    const uint32_t kc = *reinterpret_cast<const uint32_t*>(p.k_codes + row * (D / 2) + ch.c * 4);
-    const uint32_t vc = *reinterpret_cast<const uint32_t*>(p.v_codes + row * (D / 2) + ch.c * 4);
-    const uint32_t ks = p.k_scales[row * (D / kQ4Block) + (ch.c >> 2)];
-    const uint32_t vs = p.v_scales[row * (D / kQ4Block) + (ch.c >> 2)];
+    const int64_t co = code_at(p.rows, sl, ch), so = scale_at(p.rows, sl, ch);
+    const uint32_t kc = *reinterpret_cast<const uint32_t*>(p.k_codes + co);
+    const uint32_t vc = *reinterpret_cast<const uint32_t*>(p.v_codes + co);
+    const uint32_t ks = p.k_scales[so];
+    const uint32_t vs = p.v_scales[so];
     const int64_t dst = ((int64_t)(t0 + ch.t) * per_tok + ch.of_token(cpr)) * 8;
     st16(k_out + dst, q4_unpack8<E>(kc, q4_scale_value(ks)));
     st16(v_out + dst, q4_unpack8<E>(vc, q4_scale_value(vs)));
@@ -236,17 +245,26 @@ int check_rows(int rows, int64_t stride, int num_blocks, int kv_heads, int head_
   FE_CHECK_ARG(stride % 8 == 0 && stride >= (int64_t)kv_heads * head_dim);
   return FE_OK;
 }
-int check_pools(const Q4Pools& p) {
+// The pools as a caller gives them (strides null: dense), and as the kernels take them
+struct PoolArgs {
+  const void *k_codes, *k_scales, *v_codes, *v_scales;
+  const fe_kv4_strides* strides;
+};
+int check_pools(const PoolArgs& a, int num_blocks, int kv_heads, int head_dim, int block_size,
+                Q4Pools& p) {
+  p = Q4Pools{(uint8_t*)a.k_codes, (uint8_t*)a.k_scales, (uint8_t*)a.v_codes,
+              (uint8_t*)a.v_scales, {}};
   FE_CHECK_ARG(p.k_codes && p.k_scales && p.v_codes && p.v_scales);
   FE_CHECK_ARG(aligned_to(p.k_codes, 16) && aligned_to(p.v_codes, 16));
-  return FE_OK;
+  return q4_layout(a.strides, num_blocks, kv_heads, head_dim, block_size, p.rows);
 }
 
 template <class E, class Slots>
-int write_rows(const void* k_new, const void* v_new, int64_t stride, const Q4Pools& p,
+int write_rows(const void* k_new, const void* v_new, int64_t stride, const PoolArgs& args,
                int num_blocks, const Slots& slots, int rows, int kv_heads, int head_dim,
                int block_size, fe_stream_t stream) {
-  if (int rc = check_pools(p)) return rc;
+  Q4Pools p;
+  if (int rc = check_pools(args, num_blocks, kv_heads, head_dim, block_size, p)) return rc;
   FE_CHECK_ARG(k_new && v_new && aligned_to(k_new, 16) && aligned_to(v_new, 16));
   const int per_wg = tokens_per_wg(kv_heads * (head_dim / 8));
   hipLaunchKernelGGL((write_kv4_kernel<E, Slots>), dim3((rows + per_wg - 1) / per_wg),
@@ -256,36 +274,32 @@ int write_rows(const void* k_new, const void* v_new, int64_t stride, const Q4Poo
   return FE_LAUNCH_STATUS();
 }
 
-inline Q4Pools pools(const void* kc, const void* ks, const void* vc, const void* vs) {
-  return Q4Pools{(uint8_t*)kc, (uint8_t*)ks, (uint8_t*)vc, (uint8_t*)vs};
-}
-
 template <class E>
-int write_slots(const void* k_new, const void* v_new, int64_t stride, const Q4Pools& p,
+int write_slots(const void* k_new, const void* v_new, int64_t stride, const PoolArgs& args,
                 int num_blocks, const int32_t* slot_block, const int32_t* slot_offset, int rows,
                 int kv_heads, int head_dim, int block_size, fe_stream_t stream) {
   if (int rc = check_rows(rows, stride, num_blocks, kv_heads, head_dim, block_size)) return rc;
   if (rows == 0) return FE_OK;
   FE_CHECK_ARG(slot_block && slot_offset);
-  return write_rows<E>(k_new, v_new, stride, p, num_blocks, SlotArrays{slot_block, slot_offset},
+  return write_rows<E>(k_new, v_new, stride, args, num_blocks, SlotArrays{slot_block, slot_offset},
                        rows, kv_heads, head_dim, block_size, stream);
 }
 
 template <class E>
-int write_decode(const void* k_new, const void* v_new, int64_t stride, const Q4Pools& p,
+int write_decode(const void* k_new, const void* v_new, int64_t stride, const PoolArgs& args,
                  int num_blocks, const int32_t* tables, int table_stride, const int32_t* ctx,
                  int batch, int kv_heads, int head_dim, int block_size, fe_stream_t stream) {
   if (int rc = check_rows(batch, stride, num_blocks, kv_heads, head_dim, block_size)) return rc;
   FE_CHECK_ARG(table_stride > 0);
   if (batch == 0) return FE_OK;
   FE_CHECK_ARG(tables && ctx);
-  return write_rows<E>(k_new, v_new, stride, p, num_blocks,
+  return write_rows<E>(k_new, v_new, stride, args, num_blocks,
                        SlotDecode{tables, ctx, table_stride, log2_exact(block_size)}, batch,
                        kv_heads, head_dim, block_size, stream);
 }
 
 template <class E>
-int write_ragged(const void* k_new, const void* v_new, int64_t stride, const Q4Pools& p,
+int write_ragged(const void* k_new, const void* v_new, int64_t stride, const PoolArgs& args,
                  int num_blocks, const int32_t* tables, int table_stride, const int32_t* q_off,
                  const int32_t* ctx, int num_seqs, int total, int kv_heads, int head_dim,
                  int block_size, fe_stream_t stream) {
@@ -293,13 +307,13 @@ int write_ragged(const void* k_new, const void* v_new, int64_t stride, const Q4P
   FE_CHECK_ARG(num_seqs >= 0 && table_stride > 0);
   if (num_seqs == 0 || total == 0) return FE_OK;
   FE_CHECK_ARG(tables && q_off && ctx);
-  return write_rows<E>(k_new, v_new, stride, p, num_blocks,
+  return write_rows<E>(k_new, v_new, stride, args, num_blocks,
                        SlotRagged{tables, q_off, ctx, num_seqs, table_stride, log2_exact(block_size)},
                        total, kv_heads, head_dim, block_size, stream);
 }
 
 template <class E>
-int gather(const Q4Pools& p, int num_blocks, const int32_t* tables, int table_stride,
+int gather(const PoolArgs& args, int num_blocks, const int32_t* tables, int table_stride,
            const int32_t* ctx, const int32_t* out_offsets, void* k_out, void* v_out, int batch,
            int total, int kv_heads, int head_dim, int block_size, fe_stream_t stream) {
   if (int rc = check_rows(total, (int64_t)kv_heads * head_dim, num_blocks, kv_heads, head_dim,
@@ -307,7 +321,8 @@ int gather(const Q4Pools& p, int num_blocks, const int32_t* tables, int table_st
     return rc;
   FE_CHECK_ARG(batch >= 0 && table_stride > 0);
   if (batch == 0 || total == 0) return FE_OK;
-  if (int rc = check_pools(p)) return rc;
+  Q4Pools p;
+  if (int rc = check_pools(args, num_blocks, kv_heads, head_dim, block_size, p)) return rc;
   FE_CHECK_ARG(tables && ctx && out_offsets && k_out && v_out && aligned_to(k_out, 16) &&
                aligned_to(v_out, 16));
   const int per_wg = tokens_per_wg(kv_heads * (head_dim / 8));
@@ -320,45 +335,51 @@ int gather(const Q4Pools& p, int num_blocks, const int32_t* tables, int table_st
 
 }  // namespace
 
-// The fp16 form and its bf16 twin of each entry point.
-#define FE_KV4_FORMS(SUFFIX, E)                                                                    \
-  extern "C" int fe_write_kv4##SUFFIX(                                                             \
+// The fp16 form and its bf16 twin of each entry point, and the forms that take strides.
+#define FE_KV4_FORMS(STRIDED, SUFFIX, E, STRIDES_PARAM, STRIDES)                                   \
+  extern "C" int fe_write_kv4##STRIDED##SUFFIX(                                                    \
       const void* k_new, const void* v_new, int64_t new_token_stride, void* k_codes,               \
-      void* k_scales, void* v_codes, void* v_scales, int num_blocks, const int32_t* slot_block,    \
-      const int32_t* slot_offset, int num_tokens, int kv_heads, int head_dim, int block_size,      \
-      fe_stream_t stream) {                                                                        \
+      void* k_scales, void* v_codes, void* v_scales, STRIDES_PARAM int num_blocks,                 \
+      const int32_t* slot_block, const int32_t* slot_offset, int num_tokens, int kv_heads,         \
+      int head_dim, int block_size, fe_stream_t stream) {                                          \
     return write_slots<E>(k_new, v_new, new_token_stride,                                          \
-                          pools(k_codes, k_scales, v_codes, v_scales), num_blocks, slot_block,     \
-                          slot_offset, num_tokens, kv_heads, head_dim, block_size, stream);        \
+                          PoolArgs{k_codes, k_scales, v_codes, v_scales, STRIDES}, num_blocks,     \
+                          slot_block, slot_offset, num_tokens, kv_heads, head_dim, block_size,     \
+                          stream);                                                                 \
   }                                                                                                \
-  extern "C" int fe_write_kv4_decode##SUFFIX(                                                      \
+  extern "C" int fe_write_kv4_decode##STRIDED##SUFFIX(                                             \
       const void* k_new, const void* v_new, int64_t new_batch_stride, void* k_codes,               \
-      void* k_scales, void* v_codes, void* v_scales, int num_blocks, const int32_t* block_tables,  \
-      int table_stride, const int32_t* context_lens, int batch, int kv_heads, int head_dim,        \
-      int block_size, fe_stream_t stream) {                                                        \
-    return write_decode<E>(k_new, v_new, new_batch_stride,                                         \
-                           pools(k_codes, k_scales, v_codes, v_scales), num_blocks, block_tables,  \
-                           table_stride, context_lens, batch, kv_heads, head_dim, block_size,      \
-                           stream);                                                                \
-  }                                                                                                \
-  extern "C" int fe_write_kv4_ragged##SUFFIX(                                                      \
-      const void* k_new, const void* v_new, int64_t new_token_stride, void* k_codes,               \
-      void* k_scales, void* v_codes, void* v_scales, int num_blocks, const int32_t* block_tables,  \
-      int table_stride, const int32_t* q_offsets, const int32_t* context_lens, int num_seqs,       \
-      int total_tokens, int kv_heads, int head_dim, int block_size, fe_stream_t stream) {          \
-    return write_ragged<E>(k_new, v_new, new_token_stride,                                         \
-                           pools(k_codes, k_scales, v_codes, v_scales), num_blocks, block_tables,  \
-                           table_stride, q_offsets, context_lens, num_seqs, total_tokens,          \
-                           kv_heads, head_dim, block_size, stream);                                \
-  }                                                                                                \
-  extern "C" int fe_gather_kv4##SUFFIX(                                                            \
-      const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,        \
-      int num_blocks, const int32_t* block_tables, int table_stride, const int32_t* context_lens,  \
-      const int32_t* out_offsets, void* k_out, void* v_out, int batch, int total_tokens,           \
+      void* k_scales, void* v_codes, void* v_scales, STRIDES_PARAM int num_blocks,                 \
+      const int32_t* block_tables, int table_stride, const int32_t* context_lens, int batch,       \
       int kv_heads, int head_dim, int block_size, fe_stream_t stream) {                            \
-    return gather<E>(pools(k_codes, k_scales, v_codes, v_scales), num_blocks, block_tables,        \
-                     table_stride, context_lens, out_offsets, k_out, v_out, batch, total_tokens,   \
-                     kv_heads, head_dim, block_size, stream);                                      \
+    return write_decode<E>(k_new, v_new, new_batch_stride,                                         \
+                           PoolArgs{k_codes, k_scales, v_codes, v_scales, STRIDES}, num_blocks,    \
+                           block_tables, table_stride, context_lens, batch, kv_heads, head_dim,    \
+                           block_size, stream);                                                    \
+  }                                                                                                \
+  extern "C" int fe_write_kv4_ragged##STRIDED##SUFFIX(                                             \
+      const void* k_new, const void* v_new, int64_t new_token_stride, void* k_codes,               \
+      void* k_scales, void* v_codes, void* v_scales, STRIDES_PARAM int num_blocks,                 \
+      const int32_t* block_tables, int table_stride, const int32_t* q_offsets,                     \
+      const int32_t* context_lens, int num_seqs, int total_tokens, int kv_heads, int head_dim,     \
+      int block_size, fe_stream_t stream) {                                                        \
+    return write_ragged<E>(k_new, v_new, new_token_stride,                                         \
+                           PoolArgs{k_codes, k_scales, v_codes, v_scales, STRIDES}, num_blocks,    \
+                           block_tables, table_stride, q_offsets, context_lens, num_seqs,          \
+                           total_tokens, kv_heads, head_dim, block_size, stream);                  \
+  }                                                                                                \
+  extern "C" int fe_gather_kv4##STRIDED##SUFFIX(                                                   \
+      const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,        \
+      STRIDES_PARAM int num_blocks, const int32_t* block_tables, int table_stride,                 \
+      const int32_t* context_lens, const int32_t* out_offsets, void* k_out, void* v_out,           \
+      int batch, int total_tokens, int kv_heads, int head_dim, int block_size,                     \
+      fe_stream_t stream) {                                                                        \
+    return gather<E>(PoolArgs{k_codes, k_scales, v_codes, v_scales, STRIDES}, num_blocks,          \
+                     block_tables, table_stride, context_lens, out_offsets, k_out, v_out, batch,   \
+                     total_tokens, kv_heads, head_dim, block_size, stream);                        \
   }
-FE_KV4_FORMS(, Fp16)
-FE_KV4_FORMS(_bf16, Bf16)
+#define FE_STRIDES_PARAM const fe_kv4_strides *strides,
+FE_KV4_FORMS(, , Fp16, , nullptr)
+FE_KV4_FORMS(, _bf16, Bf16, , nullptr)
+FE_KV4_FORMS(_strided, , Fp16, FE_STRIDES_PARAM, strides)
+FE_KV4_FORMS(_strided, _bf16, Bf16, FE_STRIDES_PARAM, strides)

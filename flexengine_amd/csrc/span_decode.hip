@@ -70,11 +70,13 @@ struct SpanArgs {
   int max_len;
   float scale_log2;
   Span span;
+  Q4Layout rows4;  // 4-bit pools
 };
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSc1 = 16;  // buffer-instruction cache policy: sc1 (device-coherent)
+constexpr uint32_t kPastEnd = 0x7ffffff0u;  // an offset past every buffer: loads give zeros
 
 __device__ __forceinline__ void store_coherent(float* p, float v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -116,7 +118,7 @@ struct Rows16 {
     dr = a.dr;
   }
   static __device__ __forceinline__ int q_dim(int s) { return (4 * s + (lane_id() >> 4)) * 8; }
-  static __device__ __forceinline__ int pool_row(const SpanArgs& a, int hp, int blk, int off) {
+  static __device__ __forceinline__ int pool_row(const SpanArgs& a, int blk, int off) {
     return blk * a.BS + off;
   }
   __device__ __forceinline__ void load(int row, int rows, Tile& t) const {
@@ -199,51 +201,59 @@ struct Rows4 {
   const uint8_t* kc;
   const uint8_t* vc;
   const uint8_t* ks;
-  const uint8_t* vs;
-  int dr;
+  const uint8_t* vs;  // of the head
+  Q4Layout at;
+  int dr, bs_log2;
 
-  __device__ __forceinline__ void init(const SpanArgs& a, int) {
-    kc = (const uint8_t*)a.k_pool;
-    vc = (const uint8_t*)a.v_pool;
-    ks = a.k_scales;
-    vs = a.v_scales;
+  __device__ __forceinline__ void init(const SpanArgs& a, int hp) {
+    at = a.rows4;
+    kc = (const uint8_t*)a.k_pool + at.code_offset(hp);
+    vc = (const uint8_t*)a.v_pool + at.code_offset(hp);
+    ks = a.k_scales + at.scale_offset(hp);
+    vs = a.v_scales + at.scale_offset(hp);
     dr = a.dr;
+    bs_log2 = a.bs_log2;
   }
   static __device__ __forceinline__ int dim0() { return (lane_id() >> 4) * (D / 4); }
   static __device__ __forceinline__ int q_dim(int s) { return dim0() + 8 * s; }
-  static __device__ __forceinline__ int pool_row(const SpanArgs& a, int hp, int blk, int off) {
-    return (blk * (a.Hkv / a.hdiv) + hp) * a.BS + off;
+  static __device__ __forceinline__ int pool_row(const SpanArgs& a, int blk, int off) {
+    return blk * a.BS + off;
   }
+  __device__ __forceinline__ int block_of(int row) const { return row >> bs_log2; }
+  __device__ __forceinline__ int offset_of(int row) const { return row & ((1 << bs_log2) - 1); }
   __device__ __forceinline__ void load_half(const uint8_t* codes, const uint8_t* scales, int row,
                                             int rows, Half& t) const {
-    const int cb = dr / 2, sb = dr / kQ4Block;
-    rows = rows > 0 ? rows : 0;
-    const __amdgpu_buffer_rsrc_t cr = uniform_rsrc(codes + (int64_t)row * cb, rows * cb);
-    const __amdgpu_buffer_rsrc_t sr = uniform_rsrc(scales + (int64_t)row * sb, rows * sb);
+    // from the first row to the end of the last one, nothing without rows (0 <= rows <= 16);
+    // between them may be other heads' rows
+    const int cs = (int)at.code_token * 16, ss = (int)at.scale_token;
+    const int blk = block_of(row), off = offset_of(row);
+    const __amdgpu_buffer_rsrc_t cr =
+        uniform_rsrc(codes + at.code_row(blk, off), max(rows * cs - (cs - dr / 2), 0));
+    const __amdgpu_buffer_rsrc_t sr = uniform_rsrc(
+        scales + at.scale_row(blk, off), max(rows * ss - (ss - dr / kQ4Block), 0));
     const int n = lane_id() & 15;
-    const uint32_t co = (uint32_t)(n * cb + dim0() / 2);
-    const uint32_t so = (uint32_t)(n * sb + dim0() / kQ4Block);
-#pragma unroll
-    for (int j = 0; j < NW; ++j) t.c[j] = 0;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) t.s[j] = 0;
+    const uint32_t co = (uint32_t)(n * cs + dim0() / 2);
+    const uint32_t so = (uint32_t)(n * ss + dim0() / kQ4Block);
+    // (blocks past the real row come from past the descriptor's end: zeros)
     if constexpr (D == 64) {
-      if (!PAD || dim0() < dr) {
-        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(cr, co, 0, kPagePolicy));
-        t.c[0] = x[0];
-        t.c[1] = x[1];
-        t.s[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sr, so, 0, kPagePolicy);
-      }
+      const bool on = !PAD || dim0() < dr;
+      const u32x2 x = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(cr, on ? co : kPastEnd, 0, kPagePolicy));
+      t.c[0] = x[0];
+      t.c[1] = x[1];
+      t.s[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sr, on ? so : kPastEnd, 0, kPagePolicy);
     } else {
 #pragma unroll
-      for (int j = 0; j < NS; ++j)
-        if (!PAD || dim0() + 32 * j < dr) {
-          const u32x4 x = __builtin_bit_cast(
-              u32x4, __builtin_amdgcn_raw_buffer_load_b128(cr, co + 16 * j, 0, kPagePolicy));
+      for (int j = 0; j < NS; ++j) {
+        const bool on = !PAD || dim0() + 32 * j < dr;
+        const u32x4 x = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(cr, on ? co + 16 * j : kPastEnd, 0,
+                                                         kPagePolicy));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) t.c[4 * j + i] = x[i];
-          t.s[j] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sr, so + j, 0, kPagePolicy);
-        }
+        for (int i = 0; i < 4; ++i) t.c[4 * j + i] = x[i];
+        t.s[j] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sr, on ? so + j : kPastEnd, 0,
+                                                              kPagePolicy);
+      }
     }
   }
   __device__ __forceinline__ void load(int row, int rows, Tile& t) const {
@@ -310,20 +320,20 @@ struct Rows4 {
   }
   __device__ __forceinline__ void store_new(const SpanArgs& a, const NewRow& nr, int row, int r) const {
     if ((lane_id() & 15) != r) return;
-    const int cb = dr / 2, sb = dr / kQ4Block;
-    const int64_t co = (int64_t)(row + r) * cb + dim0() / 2;
-    const int64_t so = (int64_t)(row + r) * sb + dim0() / kQ4Block;
+    const int blk = block_of(row), off = offset_of(row) + r;  // (a tile lies in one page)
+    const uint64_t co = at.code_row(blk, off) + dim0() / 2;
+    const uint64_t so = at.scale_row(blk, off) + dim0() / kQ4Block;
 #pragma unroll
     for (int w = 0; w < NW; ++w)
       if (!PAD || dim0() + 8 * w < dr) {
-        *reinterpret_cast<uint32_t*>((uint8_t*)a.k_pool + co + 4 * w) = nr.k.c[w];
-        *reinterpret_cast<uint32_t*>((uint8_t*)a.v_pool + co + 4 * w) = nr.v.c[w];
+        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(kc) + co + 4 * w) = nr.k.c[w];
+        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(vc) + co + 4 * w) = nr.v.c[w];
       }
 #pragma unroll
     for (int j = 0; j < NS; ++j)
       if ((!PAD || dim0() + 32 * j < dr) && dim0() % kQ4Block == 0) {
-        a.k_scales[so + j] = (uint8_t)nr.k.s[j];
-        a.v_scales[so + j] = (uint8_t)nr.v.s[j];
+        const_cast<uint8_t*>(ks)[so + j] = (uint8_t)nr.k.s[j];
+        const_cast<uint8_t*>(vs)[so + j] = (uint8_t)nr.v.s[j];
       }
   }
 };
@@ -668,7 +678,7 @@ void span_decode_kernel(const SpanArgs a) {
       blk = a.tables[(int64_t)b * a.W + (tok >> a.bs_log2)];
     }
     core.tok_vec = tok;
-    core.row_vec = Rows::pool_row(a, hp, clamp_block(blk, a.NB), tok & (a.BS - 1));
+    core.row_vec = Rows::pool_row(a, clamp_block(blk, a.NB), tok & (a.BS - 1));
 #pragma unroll
     for (int s = 0; s < C::NK; ++s) {
       const int d = Rows::q_dim(s);
@@ -829,7 +839,7 @@ int launch_dim(const SpanArgs& a, hipStream_t s) {
 template <class E, bool Q4>
 int span_decode(const void* q, int64_t q_stride, void* out, const void* k_new, const void* v_new,
                 int64_t new_stride, void* k_pool, void* k_scales, void* v_pool, void* v_scales,
-                int num_blocks, const int32_t* tables, int table_stride, const int32_t* ctx,
+                const fe_kv4_strides* strides, int num_blocks, const int32_t* tables, int table_stride, const int32_t* ctx,
                 void* workspace, size_t workspace_bytes, int batch, int hq, int hkv, int d, int bs,
                 float scale, int window, int sinks, int target_splits, fe_stream_t stream) {
   FE_CHECK_ARG(batch >= 0 && hq > 0 && hkv > 0 && d > 0 && num_blocks > 0 && table_stride > 0 &&
@@ -845,7 +855,7 @@ int span_decode(const void* q, int64_t q_stride, void* out, const void* k_new, c
   if ((int64_t)batch * hkv_v > kMaxTickets) return FE_ERR_UNSUPPORTED;
   if ((int64_t)table_stride * bs > kMaxContext) return FE_ERR_UNSUPPORTED;
   // pool rows are 32-bit in the kernels, and so are the offsets within a tile's 16 rows
-  if ((int64_t)num_blocks * bs * (Q4 ? hkv : 1) >= ((int64_t)1 << 31) ||
+  if ((int64_t)num_blocks * bs >= ((int64_t)1 << 31) ||
       (int64_t)hkv * d >= ((int64_t)1 << 25))
     return FE_ERR_UNSUPPORTED;
   const int max_len = table_stride * bs;
@@ -860,7 +870,11 @@ int span_decode(const void* q, int64_t q_stride, void* out, const void* k_new, c
   const int per16 = kIsF32<E> ? 4 : 8;
   FE_CHECK_ARG(q_stride % per16 == 0 && q_stride >= (int64_t)hq * d);
   FE_CHECK_ARG(aligned16(q) && aligned16(out) && aligned16(k_pool) && aligned16(v_pool));
-  if (Q4) FE_CHECK_ARG(k_scales && v_scales);
+  Q4Layout rows4{};
+  if (Q4) {
+    FE_CHECK_ARG(k_scales && v_scales);
+    if (int rc = q4_layout(strides, num_blocks, hkv, d, bs, rows4)) return rc;
+  }
   if (k_new)
     FE_CHECK_ARG(aligned16(k_new) && aligned16(v_new) && new_stride % per16 == 0 &&
                  new_stride >= (int64_t)hkv * d);
@@ -897,6 +911,7 @@ int span_decode(const void* q, int64_t q_stride, void* out, const void* k_new, c
   a.max_len = max_len;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, window > 0 ? sinks : 0};
+  a.rows4 = rows4;
   return launch_dim<E, Q4>(a, (hipStream_t)stream);
 }
 
@@ -922,7 +937,7 @@ extern "C" size_t fe_span_decode_workspace_size(int batch, int num_q_heads, int 
       int head_dim, int block_size, float scale, int window, int sinks, int target_splits,        \
       fe_stream_t stream) {                                                                       \
     return span_decode<E, false>(q, q_batch_stride, out, k_new, v_new, new_batch_stride, k_pool,  \
-                                 nullptr, v_pool, nullptr, num_blocks, block_tables,              \
+                                 nullptr, v_pool, nullptr, nullptr, num_blocks, block_tables,     \
                                  table_stride, context_lens, workspace, workspace_bytes, batch,   \
                                  num_q_heads, kv_heads, head_dim, block_size, scale, window,      \
                                  sinks, target_splits, stream);                                   \
@@ -931,19 +946,22 @@ FE_WINDOW_DECODE(, Fp16)
 FE_WINDOW_DECODE(_bf16, Bf16)
 FE_WINDOW_DECODE(_f32, F32)
 
-#define FE_KV4_DECODE(SUFFIX, E)                                                                  \
+#define FE_KV4_DECODE(SUFFIX, E, STRIDES_PARAM, STRIDES)                                          \
   extern "C" int fe_paged_decode_kv4##SUFFIX(                                                     \
       const void* q, int64_t q_batch_stride, void* out, const void* k_new, const void* v_new,     \
       int64_t new_batch_stride, void* k_codes, void* k_scales, void* v_codes, void* v_scales,     \
-      int num_blocks, const int32_t* block_tables, int table_stride,                              \
+      STRIDES_PARAM int num_blocks, const int32_t* block_tables, int table_stride,                \
       const int32_t* context_lens, void* workspace, size_t workspace_bytes, int batch,            \
       int num_q_heads, int kv_heads, int head_dim, int block_size, float scale, int window,       \
       int sinks, int target_splits, fe_stream_t stream) {                                         \
     return span_decode<E, true>(q, q_batch_stride, out, k_new, v_new, new_batch_stride, k_codes,  \
-                                k_scales, v_codes, v_scales, num_blocks, block_tables,            \
+                                k_scales, v_codes, v_scales, STRIDES, num_blocks, block_tables,   \
                                 table_stride, context_lens, workspace, workspace_bytes, batch,    \
                                 num_q_heads, kv_heads, head_dim, block_size, scale, window,       \
                                 sinks, target_splits, stream);                                    \
   }
-FE_KV4_DECODE(, Fp16)
-FE_KV4_DECODE(_bf16, Bf16)
+#define FE_STRIDES_PARAM const fe_kv4_strides *strides,
+FE_KV4_DECODE(, Fp16, , nullptr)
+FE_KV4_DECODE(_bf16, Bf16, , nullptr)
+FE_KV4_DECODE(_strided, Fp16, FE_STRIDES_PARAM, strides)
+FE_KV4_DECODE(_strided_bf16, Bf16, FE_STRIDES_PARAM, strides)

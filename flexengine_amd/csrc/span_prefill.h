@@ -79,6 +79,7 @@ struct SpanPrefill {
   int dr;            // the real head_dim (PAD: below D)
   float scale_log2;
   Span span;
+  Q4Layout rows4;  // 4-bit pools
 };
 
 // The 16-key tiles that a run of query rows walks: those of the sinks, then those from the one
@@ -525,7 +526,8 @@ struct Stage4 {
     }
   }
   __device__ __forceinline__ void load(const SpanPrefill& a, const SpanWalk& wk, int h, int j) {
-    const int cb = a.dr / 2, sb = a.dr / kQ4Block;
+    const Q4Layout& at = a.rows4;
+    const int sb = a.dr / kQ4Block;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = chunk(i), key = key_at(wk, j, i), blk = c % BPR;
@@ -533,12 +535,11 @@ struct Stage4 {
       codes[i] = span_u32x4{0, 0, 0, 0};
       scale[i] = kQ4ScaleLow;
       if (c < CHUNKS && (!PAD || blk < sb) && wk.sees(key)) {
-        const int64_t row =
-            ((int64_t)clamp_block(id[i], a.NB) * a.Hkv + h) * a.BS + (key & (a.BS - 1));
-        const uint8_t* cp = (const uint8_t*)(is_v ? a.v_pool : a.k_pool);
-        const uint8_t* sp = is_v ? a.v_scales : a.k_scales;
-        codes[i] = *reinterpret_cast<const span_u32x4*>(cp + row * cb + blk * 16);
-        scale[i] = sp[row * sb + blk];
+        const int page = clamp_block(id[i], a.NB), off = key & (a.BS - 1);
+        const uint8_t* cp = (const uint8_t*)(is_v ? a.v_pool : a.k_pool) + at.code_offset(h);
+        const uint8_t* sp = (is_v ? a.v_scales : a.k_scales) + at.scale_offset(h);
+        codes[i] = *reinterpret_cast<const span_u32x4*>(cp + at.code_row(page, off) + blk * 16);
+        scale[i] = sp[at.scale_row(page, off) + blk];
       }
     }
   }
@@ -763,7 +764,8 @@ int span_launch(const SpanPrefill& a, const SpanShape& p, hipStream_t s) {
 // Checks and launch that the 16-bit and the 4-bit forms share
 template <class E, bool Q4>
 int span_prefill(const void* q, void* out, const void* k_pool, const void* k_scales,
-                 const void* v_pool, const void* v_scales, int num_blocks, const int32_t* tables,
+                 const void* v_pool, const void* v_scales, const fe_kv4_strides* strides,
+                 int num_blocks, const int32_t* tables,
                  int table_stride, const int32_t* q_off, const int32_t* ctx, int num_seqs,
                  int total_q, int hq, int hkv, int d, int bs, float scale, int window, int sinks,
                  void* workspace, size_t workspace_bytes, fe_stream_t stream) {
@@ -781,7 +783,11 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
     return FE_ERR_UNSUPPORTED;
   if (num_seqs == 0 || total_q == 0) return FE_OK;
   FE_CHECK_ARG(q && out && k_pool && v_pool && tables && q_off && ctx);
-  if (Q4) FE_CHECK_ARG(k_scales && v_scales);
+  Q4Layout rows4{};
+  if (Q4) {
+    FE_CHECK_ARG(k_scales && v_scales);
+    if (int rc = q4_layout(strides, num_blocks, hkv, d, bs, rows4)) return rc;
+  }
   const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   FE_CHECK_ARG(aligned(q) && aligned(out) && aligned(k_pool) && aligned(v_pool));
   const SpanShape p = span_shape(num_seqs, total_q, hq, hkv, d, window, Q4);
@@ -815,6 +821,7 @@ int span_prefill(const void* q, void* out, const void* k_pool, const void* k_sca
   a.dr = d;
   a.scale_log2 = scale * kLog2e;
   a.span = Span{window, window > 0 ? sinks : 0};
+  a.rows4 = rows4;
   const hipStream_t s = (hipStream_t)stream;
   if (d == 64) return span_launch<64, E, Q4, false>(a, p, s);
   if (d == 128) return span_launch<128, E, Q4, false>(a, p, s);

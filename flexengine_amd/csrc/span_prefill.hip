@@ -230,7 +230,7 @@ extern "C" size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int 
       const int32_t* context_lens, int num_seqs, int total_q, int num_q_heads, int kv_heads,      \
       int head_dim, int block_size, float scale, int window, int sinks, void* workspace,          \
       size_t workspace_bytes, fe_stream_t stream) {                                               \
-    return span_prefill<E, false>(q, out, k_pool, nullptr, v_pool, nullptr, num_blocks,           \
+    return span_prefill<E, false>(q, out, k_pool, nullptr, v_pool, nullptr, nullptr, num_blocks,  \
                                   block_tables, table_stride, q_offsets, context_lens, num_seqs,  \
                                   total_q, num_q_heads, kv_heads, head_dim, block_size, scale,    \
                                   window, sinks, workspace, workspace_bytes, stream);             \

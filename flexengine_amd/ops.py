@@ -9,6 +9,7 @@ the workspace / output buffers or lets them come from the graph pool.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 from dataclasses import dataclass
 import functools
 import math
@@ -39,6 +40,8 @@ class Kv4Pool:
     kv_heads, block_size, head_dim / 32], both with the same leading layer dim if the pool
     holds several; dtype: the type of its rows (float16 or bfloat16).  pool[layer] is one
     layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it.
+    The dims may lie in any order in memory and apart, as long as a row's bytes are side by side
+    and its codes start at multiples of 16 bytes; the dense layout is read fastest.
     The tensors and their shapes stay as they are at the pool's first use, which checks them."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = FP16):
@@ -46,6 +49,8 @@ class Kv4Pool:
         self.scales = scales
         self.dtype = dtype
         self._checked: tuple[int, int, int, int] | None = None
+        self._strides: tuple[int, ...] | None = None  # of a pool that is not dense
+        self._c_strides = None
         self._layers: list["Kv4Pool"] | None = None
 
     @classmethod
@@ -96,7 +101,7 @@ class Kv4Pool:
             raise ValueError("4-bit pools need uint8 codes [..., head_dim / 2] and scales "
                              "[..., head_dim / 32] (head_dim a multiple of 32)")
         if not (codes.is_contiguous() and scales.is_contiguous()):
-            raise ValueError("K/V pools must be contiguous")
+            self._strides, self._c_strides = _kv4_strides(shape, codes.stride(), scales.stride())
         if scales.get_device() != codes.get_device():
             raise ValueError(f"all tensors must be on {codes.device}")
         self._checked = nb, bs, hkv, 2 * half
@@ -108,6 +113,27 @@ class Kv4Pool:
             self._layers = [Kv4Pool(c, s, self.dtype)
                             for c, s in zip(self.codes.unbind(0), self.scales.unbind(0))]
         return self._layers[layer]
+
+
+@functools.lru_cache(maxsize=256)
+def _kv4_strides(shape: tuple, codes: tuple, scales: tuple):
+    """Bytes between the blocks, heads and tokens of a 4-bit pool's codes and of its scales (0 for
+    a dim of 1), as a tuple and as the library's fe_kv4_strides, from shape and strides alone."""
+    *size, half = shape
+    got = []
+    for stride, row, unit in ((codes, half, 16), (scales, half // 16, 1)):
+        if row > 1 and stride[3] != 1:
+            raise ValueError("the bytes of a 4-bit row must be side by side")
+        stride = [0 if n == 1 else s for n, s in zip(size, stride)]
+        extent = row
+        # each stride at least what the smaller ones span: no two rows share a byte
+        for step, n in sorted(zip(stride, size)):
+            if n > 1 and step < extent or step % unit:
+                raise ValueError("the rows of 4-bit pools must lie apart, codes at multiples of "
+                                 "16 bytes")
+            extent += step * (n - 1)
+        got += stride
+    return tuple(got), (ctypes.c_int64 * 6)(*got)
 
 
 def _require_gpu(*tensors: torch.Tensor) -> torch.device:
@@ -165,6 +191,8 @@ def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
     layout = k_pool.layout()
     if v_pool.layout() != layout or v_pool.dtype != k_pool.dtype:
         raise ValueError("K and V pools must have the same shape and hold rows of the same type")
+    if v_pool._strides != k_pool._strides:
+        raise ValueError("K and V pools must have the same strides")
     return layout
 
 
@@ -177,10 +205,11 @@ def _any_pool(k_pool, v_pool) -> tuple[int, int, int, int]:
         _check_pool(k_pool, v_pool, KV_DTYPES)
 
 
-# entry points of the page movers by pool type (a pair: the 4-bit pools' forms)
+# entry points of the page movers by pool type (beside them the 4-bit pools' forms, dense and not)
 _MOVERS = {
     base + tail: ({dt: f"fe_{base}{tail}{sfx}" for dt, sfx in _MOVER_SFX.items()},
-                  {dt: f"fe_{base}4{tail}{_SFX[dt]}" for dt in DTYPES_16})
+                  {dt: f"fe_{base}4{tail}{_SFX[dt]}" for dt in DTYPES_16},
+                  {dt: f"fe_{base}4{tail}_strided{_SFX[dt]}" for dt in DTYPES_16})
     for base, tail in (("write_kv", ""), ("write_kv", "_decode"), ("write_kv", "_ragged"),
                        ("gather_kv", ""))
 }
@@ -188,15 +217,35 @@ _MOVERS = {
 
 def _mover(name: str, k_pool, v_pool) -> tuple[str, tuple]:
     """A page mover's entry point for these pools, and the pools' pointers."""
-    plain, four = _MOVERS[name]
+    plain, four, strided = _MOVERS[name]
     if isinstance(k_pool, Kv4Pool):
-        return four[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
+        names = four if k_pool._strides is None else strided
+        return names[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
     return plain[k_pool.dtype], (k_pool.data_ptr(), v_pool.data_ptr())
 
 
 def _kv4_ptrs(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple:
-    return (k_pool.codes.data_ptr(), k_pool.scales.data_ptr(), v_pool.codes.data_ptr(),
+    ptrs = (k_pool.codes.data_ptr(), k_pool.scales.data_ptr(), v_pool.codes.data_ptr(),
             v_pool.scales.data_ptr())
+    return ptrs if k_pool._strides is None else ptrs + (k_pool._c_strides,)
+
+
+# entry points of the attention calls under a window (by pool type) and over 4-bit pools
+_SPAN_CALLS = {
+    op: ({dt: f"fe_{op}_window{sfx}" for dt, sfx in _SFX.items()},
+         {dt: f"fe_{op}_kv4{_SFX[dt]}" for dt in DTYPES_16},
+         {dt: f"fe_{op}_kv4_strided{_SFX[dt]}" for dt in DTYPES_16})
+    for op in ("paged_decode", "prefill_paged")
+}
+
+
+def _span_call(op: str, k_pool, v_pool) -> tuple[str, tuple]:
+    """The entry point of an attention call for these pools, and the pools' pointers."""
+    window, four, strided = _SPAN_CALLS[op]
+    if isinstance(k_pool, Kv4Pool):
+        names = four if k_pool._strides is None else strided
+        return names[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
+    return window[k_pool.dtype], (k_pool.data_ptr(), v_pool.data_ptr())
 
 
 def check_window(window: int | None, sinks: int = 0) -> tuple[int, int]:
@@ -520,8 +569,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     """
     (dev, nb, bs, hkv, d, batch, hq, block_tables, context_lens, new_stride, out,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
-    kv4 = isinstance(k_pool, Kv4Pool)
-    if kv4 or window is not None or sinks:
+    if isinstance(k_pool, Kv4Pool) or window is not None or sinks:
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no decode plan")
@@ -530,10 +578,9 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
             workspace = decode_workspace(dev, _pure_size(
                 "fe_span_decode_workspace_size", batch, hq, hkv, d, block_tables.shape[1] * bs,
                 target_splits), kind="span_decode")
-        pools = _kv4_ptrs(k_pool, v_pool) if kv4 else (k_pool.data_ptr(), v_pool.data_ptr())
-        _lib.call(("fe_paged_decode_kv4" if kv4 else "fe_paged_decode_window") + _SFX[q.dtype],
-                  q.data_ptr(), q.stride(0), out.data_ptr(), _ptr(k_new), _ptr(v_new), new_stride,
-                  *pools, nb, block_tables.data_ptr(), block_tables.shape[1],
+        name, pools = _span_call("paged_decode", k_pool, v_pool)
+        _lib.call(name, q.data_ptr(), q.stride(0), out.data_ptr(), _ptr(k_new), _ptr(v_new),
+                  new_stride, *pools, nb, block_tables.data_ptr(), block_tables.shape[1],
                   context_lens.data_ptr(), workspace.data_ptr(),
                   workspace.numel() * workspace.element_size(), batch, hq, hkv, d, bs,
                   float(scale), window, sinks, int(target_splits), _stream(dev))
@@ -738,8 +785,7 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    kv4 = isinstance(k_pool, Kv4Pool)
-    if kv4 or window is not None or sinks:
+    if isinstance(k_pool, Kv4Pool) or window is not None or sinks:
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no prefill plan")
@@ -747,9 +793,8 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         if workspace is None:
             workspace = decode_workspace(dev, int(_lib.load().fe_span_prefill_workspace_size(
                 num_seqs, total_q, hq, hkv, d)), kind="span_prefill")
-        pools = _kv4_ptrs(k_pool, v_pool) if kv4 else (k_pool.data_ptr(), v_pool.data_ptr())
-        _lib.call(("fe_prefill_paged_kv4" if kv4 else "fe_prefill_paged_window") + _SFX[q.dtype],
-                  q.data_ptr(), out.data_ptr(), *pools, nb, block_tables.data_ptr(),
+        name, pools = _span_call("prefill_paged", k_pool, v_pool)
+        _lib.call(name, q.data_ptr(), out.data_ptr(), *pools, nb, block_tables.data_ptr(),
                   block_tables.shape[1], q_offsets.data_ptr(), context_lens.data_ptr(), num_seqs,
                   total_q, hq, hkv, d, bs, float(scale), window, sinks, workspace.data_ptr(),
                   workspace.numel() * workspace.element_size(), _stream(dev))

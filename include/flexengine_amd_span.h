@@ -16,6 +16,7 @@
  *   codes   uint8 [num_blocks, kv_heads, block_size, head_dim / 2], 16-byte aligned; dim 2i in
  *           the low half of byte i
  *   scales  uint8 [num_blocks, kv_heads, block_size, head_dim / 32]
+ * The _strided forms take the same dims in any order and with gaps between rows (fe_kv4_strides).
  * A write takes the smallest power of two 2^e with max|x| <= 7 * 2^e, -23 <= e <= 13 (fp16
  * rows) or 125 (bf16 rows), and rounds to the nearest code, ties to the even one.  Every value
  * is exact in the rows' type.  fp16 magnitudes above 49152 are held as 49152; a block with an
@@ -35,6 +36,18 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/*
+ * Where the rows of 4-bit pools are: bytes between blocks, KV heads and tokens, of the codes
+ * (multiples of 16) and of the scales; K's and V's alike.  The bytes of a row are side by side
+ * and rows lie apart: each stride is at least what the smaller ones span (else
+ * FE_ERR_INVALID_ARGUMENT); block strides below 2^36 and 2^32, token strides below 2^26.  The
+ * stride of a dim of size 1 counts for nothing.  Null: the layout above.
+ */
+typedef struct {
+  int64_t codes[3];
+  int64_t scales[3];
+} fe_kv4_strides;
 
 /*
  * Page writes into 4-bit pools: fe_write_kv, fe_write_kv_decode and fe_write_kv_ragged
@@ -184,6 +197,95 @@ int fe_prefill_paged_kv4_bf16(const void* q, void* out, const void* k_codes,
                               int total_q, int num_q_heads, int kv_heads, int head_dim,
                               int block_size, float scale, int window, int sinks, void* workspace,
                               size_t workspace_bytes, fe_stream_t stream);
+
+/*
+ * The forms above of 4-bit pools with strides of their own (null: those forms).  Reads cost least
+ * where the rows of a head are side by side, as in the layout above: at head_dim 128 two rows of
+ * neighbouring heads that are side by side share a cache line that both heads' reads fetch.
+ */
+int fe_write_kv4_strided(const void* k_new, const void* v_new, int64_t new_token_stride,
+                         void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                         const fe_kv4_strides* strides, int num_blocks, const int32_t* slot_block,
+                         const int32_t* slot_offset, int num_tokens, int kv_heads, int head_dim,
+                         int block_size, fe_stream_t stream);
+int fe_write_kv4_strided_bf16(const void* k_new, const void* v_new, int64_t new_token_stride,
+                              void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                              const fe_kv4_strides* strides, int num_blocks,
+                              const int32_t* slot_block, const int32_t* slot_offset, int num_tokens,
+                              int kv_heads, int head_dim, int block_size, fe_stream_t stream);
+int fe_write_kv4_decode_strided(const void* k_new, const void* v_new, int64_t new_batch_stride,
+                                void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                const fe_kv4_strides* strides, int num_blocks,
+                                const int32_t* block_tables, int table_stride,
+                                const int32_t* context_lens, int batch, int kv_heads, int head_dim,
+                                int block_size, fe_stream_t stream);
+int fe_write_kv4_decode_strided_bf16(const void* k_new, const void* v_new, int64_t new_batch_stride,
+                                     void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                     const fe_kv4_strides* strides, int num_blocks,
+                                     const int32_t* block_tables, int table_stride,
+                                     const int32_t* context_lens, int batch, int kv_heads,
+                                     int head_dim, int block_size, fe_stream_t stream);
+int fe_write_kv4_ragged_strided(const void* k_new, const void* v_new, int64_t new_token_stride,
+                                void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                const fe_kv4_strides* strides, int num_blocks,
+                                const int32_t* block_tables, int table_stride,
+                                const int32_t* q_offsets, const int32_t* context_lens, int num_seqs,
+                                int total_tokens, int kv_heads, int head_dim, int block_size,
+                                fe_stream_t stream);
+int fe_write_kv4_ragged_strided_bf16(const void* k_new, const void* v_new, int64_t new_token_stride,
+                                     void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                     const fe_kv4_strides* strides, int num_blocks,
+                                     const int32_t* block_tables, int table_stride,
+                                     const int32_t* q_offsets, const int32_t* context_lens,
+                                     int num_seqs, int total_tokens, int kv_heads, int head_dim,
+                                     int block_size, fe_stream_t stream);
+int fe_gather_kv4_strided(const void* k_codes, const void* k_scales, const void* v_codes,
+                          const void* v_scales, const fe_kv4_strides* strides, int num_blocks,
+                          const int32_t* block_tables, int table_stride,
+                          const int32_t* context_lens, const int32_t* out_offsets, void* k_out,
+                          void* v_out, int batch, int total_tokens, int kv_heads, int head_dim,
+                          int block_size, fe_stream_t stream);
+int fe_gather_kv4_strided_bf16(const void* k_codes, const void* k_scales, const void* v_codes,
+                               const void* v_scales, const fe_kv4_strides* strides, int num_blocks,
+                               const int32_t* block_tables, int table_stride,
+                               const int32_t* context_lens, const int32_t* out_offsets, void* k_out,
+                               void* v_out, int batch, int total_tokens, int kv_heads, int head_dim,
+                               int block_size, fe_stream_t stream);
+int fe_paged_decode_kv4_strided(const void* q, int64_t q_batch_stride, void* out, const void* k_new,
+                                const void* v_new, int64_t new_batch_stride, void* k_codes,
+                                void* k_scales, void* v_codes, void* v_scales,
+                                const fe_kv4_strides* strides, int num_blocks,
+                                const int32_t* block_tables, int table_stride,
+                                const int32_t* context_lens, void* workspace,
+                                size_t workspace_bytes, int batch, int num_q_heads, int kv_heads,
+                                int head_dim, int block_size, float scale, int window, int sinks,
+                                int target_splits, fe_stream_t stream);
+int fe_paged_decode_kv4_strided_bf16(const void* q, int64_t q_batch_stride, void* out,
+                                     const void* k_new, const void* v_new, int64_t new_batch_stride,
+                                     void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                     const fe_kv4_strides* strides, int num_blocks,
+                                     const int32_t* block_tables, int table_stride,
+                                     const int32_t* context_lens, void* workspace,
+                                     size_t workspace_bytes, int batch, int num_q_heads,
+                                     int kv_heads, int head_dim, int block_size, float scale,
+                                     int window, int sinks, int target_splits, fe_stream_t stream);
+int fe_prefill_paged_kv4_strided(const void* q, void* out, const void* k_codes,
+                                 const void* k_scales, const void* v_codes, const void* v_scales,
+                                 const fe_kv4_strides* strides, int num_blocks,
+                                 const int32_t* block_tables, int table_stride,
+                                 const int32_t* q_offsets, const int32_t* context_lens,
+                                 int num_seqs, int total_q, int num_q_heads, int kv_heads,
+                                 int head_dim, int block_size, float scale, int window, int sinks,
+                                 void* workspace, size_t workspace_bytes, fe_stream_t stream);
+int fe_prefill_paged_kv4_strided_bf16(const void* q, void* out, const void* k_codes,
+                                      const void* k_scales, const void* v_codes,
+                                      const void* v_scales, const fe_kv4_strides* strides,
+                                      int num_blocks, const int32_t* block_tables, int table_stride,
+                                      const int32_t* q_offsets, const int32_t* context_lens,
+                                      int num_seqs, int total_q, int num_q_heads, int kv_heads,
+                                      int head_dim, int block_size, float scale, int window,
+                                      int sinks, void* workspace, size_t workspace_bytes,
+                                      fe_stream_t stream);
 
 #ifdef __cplusplus
 }
