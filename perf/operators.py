@@ -230,7 +230,7 @@ def prepare(case, seed):
                 s[name].append((torch.zeros((nb, hkv, bs, d // 2), dtype=torch.uint8, device=DEV),
                                 torch.zeros((nb, hkv, bs, d // 32), dtype=torch.uint8, device=DEV)))
             else:
-                s[name].append(_pack(_rows(gen, (nb, bs, hkv, d), dt).transpose(1, 2).contiguous(),
+                s[name].append(_pack(_rows(gen, (nb, bs, hkv, d), dt).transpose(1, 2),
                                      case["dtype"]))
     return s
 
