@@ -469,6 +469,16 @@ def decode_workspace(device: torch.device, nbytes: int, kind: str = "decode") ->
     return ws
 
 
+def _check_workspace(workspace: torch.Tensor | None, dev: torch.device) -> None:
+    """A caller's workspace is passed on as an address and a size: its bytes have to be there."""
+    if workspace is None:
+        return
+    if workspace.get_device() != dev.index:
+        raise ValueError(f"the workspace must be on {dev}; got {workspace.device}")
+    if not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+
+
 def _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out):
     """Checks of the decode entry points; returns the normalised arguments."""
     dev = _require_gpu(q, k_pool, v_pool, block_tables, context_lens, k_new, v_new, out)
@@ -569,11 +579,11 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     """
     (dev, nb, bs, hkv, d, batch, hq, block_tables, context_lens, new_stride, out,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
+    _check_workspace(workspace, dev)
     if isinstance(k_pool, Kv4Pool) or window is not None or sinks:
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no decode plan")
-        _require_gpu(q, workspace)
         if workspace is None:
             workspace = decode_workspace(dev, _pure_size(
                 "fe_span_decode_workspace_size", batch, hq, hkv, d, block_tables.shape[1] * bs,
@@ -630,6 +640,7 @@ def paged_decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise ValueError("the shared-prefix decode has no form for 4-bit pools")
     (dev, nb, bs, hkv, d, batch, hq, block_tables, context_lens, new_stride, out,
      scale) = _decode_args(q, k_pool, v_pool, block_tables, context_lens, scale, k_new, v_new, out)
+    _check_workspace(workspace, dev)
     group_offsets = _int32(group_offsets, "group_offsets")
     group_prefix_lens = _int32(group_prefix_lens, "group_prefix_lens")
     if group_offsets.ndim != 1 or group_prefix_lens.ndim != 1 or \
@@ -764,8 +775,9 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     window: each row attends the last `window` keys up to its position and the first `sinks`
     of its sequence only (fe_prefill_paged_window).  Pools may be Kv4Pools of q's dtype
     (fe_prefill_paged_kv4).  Both want block sizes of at least 16, take no plan and have a
-    workspace of their own (fe_span_prefill_workspace_size); the per-device one unless
-    `workspace` (zero-filled uint8) is given."""
+    workspace of their own (fe_span_prefill_workspace_size).
+
+    workspace: zero-filled uint8, contiguous, on q's device; without one the per-device one."""
     dev = _require_gpu(q, k_pool, v_pool, block_tables, q_offsets, context_lens, out)
     nb, bs, hkv, d = _any_pool(k_pool, v_pool)
     if q.ndim != 3 or q.shape[2] != d or q.dtype != k_pool.dtype or not q.is_contiguous():
@@ -785,11 +797,11 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    _check_workspace(workspace, dev)
     if isinstance(k_pool, Kv4Pool) or window is not None or sinks:
         window, sinks = check_window(window, sinks)
         if plan is not None:
             raise ValueError("4-bit pools and windows take no prefill plan")
-        _require_gpu(q, workspace)
         if workspace is None:
             workspace = decode_workspace(dev, int(_lib.load().fe_span_prefill_workspace_size(
                 num_seqs, total_q, hq, hkv, d)), kind="span_prefill")
