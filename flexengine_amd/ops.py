@@ -42,16 +42,49 @@ class Kv4Pool:
     layer's, shape the plain pools' [num_blocks, block_size, kv_heads, head_dim] after it.
     The dims may lie in any order in memory and apart, as long as a row's bytes are side by side
     and its codes start at multiples of 16 bytes; the dense layout is read fastest.
-    The tensors and their shapes stay as they are at the pool's first use, which checks them."""
+    The tensors are checked at their first use; others may be assigned at any time (pool[layer]
+    then gives pools of the new ones).  Give a pool new tensors that way, not by resizing or
+    re-pointing (resize_, set_, .data) those it has."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = FP16):
-        self.codes = codes
-        self.scales = scales
-        self.dtype = dtype
+        self._codes = codes
+        self._scales = scales
+        self._dtype = dtype
+        self._forget()
+
+    def _forget(self) -> None:
+        """Drops what was found out about tensors that the pool no longer has."""
         self._checked: tuple[int, int, int, int] | None = None
         self._strides: tuple[int, ...] | None = None  # of a pool that is not dense
         self._c_strides = None
         self._layers: list["Kv4Pool"] | None = None
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @codes.setter
+    def codes(self, codes: torch.Tensor) -> None:
+        self._codes = codes
+        self._forget()
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @scales.setter
+    def scales(self, scales: torch.Tensor) -> None:
+        self._scales = scales
+        self._forget()
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self._dtype
+
+    @dtype.setter
+    def dtype(self, dtype: torch.dtype) -> None:
+        self._dtype = dtype
+        self._forget()
 
     @classmethod
     def empty(cls, shape, dtype: torch.dtype = FP16, device="cuda:0") -> "Kv4Pool":
@@ -70,30 +103,30 @@ class Kv4Pool:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     def get_device(self) -> int:
-        return self.codes.get_device()
+        return self._codes.get_device()
 
     @property
     def shape(self) -> tuple[int, ...]:
-        *lead, hkv, bs, half = self.codes.shape
+        *lead, hkv, bs, half = self._codes.shape
         return (*lead, bs, hkv, 2 * half)
 
     @property
     def ndim(self) -> int:
-        return self.codes.ndim
+        return self._codes.ndim
 
     def layout(self) -> tuple[int, int, int, int]:
         """(num_blocks, block_size, kv_heads, head_dim) of one layer's pool, its tensors checked
         (once: on every call that was 1 us of host time)."""
         if self._checked is not None:
             return self._checked
-        codes, scales = self.codes, self.scales
+        codes, scales = self._codes, self._scales
         shape = codes.shape
         if len(shape) != 4:
             raise ValueError("4-bit pools must hold one layer of [num_blocks, kv_heads, block_size]")
-        if self.dtype not in DTYPES_16:
+        if self._dtype not in DTYPES_16:
             raise ValueError("4-bit pools must hold float16 or bfloat16 rows")
         nb, hkv, bs, half = shape
         if half % 16 or scales.shape != (nb, hkv, bs, half // 16) or not (
@@ -110,8 +143,8 @@ class Kv4Pool:
     def __getitem__(self, layer: int) -> "Kv4Pool":
         """The pool of one layer (views of this one's tensors)."""
         if self._layers is None:
-            self._layers = [Kv4Pool(c, s, self.dtype)
-                            for c, s in zip(self.codes.unbind(0), self.scales.unbind(0))]
+            self._layers = [Kv4Pool(c, s, self._dtype)
+                            for c, s in zip(self._codes.unbind(0), self._scales.unbind(0))]
         return self._layers[layer]
 
 
@@ -189,7 +222,7 @@ def _check_pool4(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple[int, int, int, int]:
     if not (isinstance(k_pool, Kv4Pool) and isinstance(v_pool, Kv4Pool)):
         raise ValueError("K and V pools must both be 4-bit pools, or both tensors")
     layout = k_pool.layout()
-    if v_pool.layout() != layout or v_pool.dtype != k_pool.dtype:
+    if v_pool.layout() != layout or v_pool._dtype != k_pool._dtype:
         raise ValueError("K and V pools must have the same shape and hold rows of the same type")
     if v_pool._strides != k_pool._strides:
         raise ValueError("K and V pools must have the same strides")
@@ -220,13 +253,13 @@ def _mover(name: str, k_pool, v_pool) -> tuple[str, tuple]:
     plain, four, strided = _MOVERS[name]
     if isinstance(k_pool, Kv4Pool):
         names = four if k_pool._strides is None else strided
-        return names[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
+        return names[k_pool._dtype], _kv4_ptrs(k_pool, v_pool)
     return plain[k_pool.dtype], (k_pool.data_ptr(), v_pool.data_ptr())
 
 
 def _kv4_ptrs(k_pool: Kv4Pool, v_pool: Kv4Pool) -> tuple:
-    ptrs = (k_pool.codes.data_ptr(), k_pool.scales.data_ptr(), v_pool.codes.data_ptr(),
-            v_pool.scales.data_ptr())
+    ptrs = (k_pool._codes.data_ptr(), k_pool._scales.data_ptr(), v_pool._codes.data_ptr(),
+            v_pool._scales.data_ptr())
     return ptrs if k_pool._strides is None else ptrs + (k_pool._c_strides,)
 
 
@@ -244,7 +277,7 @@ def _span_call(op: str, k_pool, v_pool) -> tuple[str, tuple]:
     window, four, strided = _SPAN_CALLS[op]
     if isinstance(k_pool, Kv4Pool):
         names = four if k_pool._strides is None else strided
-        return names[k_pool.dtype], _kv4_ptrs(k_pool, v_pool)
+        return names[k_pool._dtype], _kv4_ptrs(k_pool, v_pool)
     return window[k_pool.dtype], (k_pool.data_ptr(), v_pool.data_ptr())
 
 
