@@ -107,6 +107,7 @@ SIGNATURES |= {
     "fe_paged_decode_kv4": (_i, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i, _p, _i, _p, _p,
                                  _sz, _i, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
     "fe_span_prefill_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "fe_span_prefill_rows": (_i, [_i] * 8),
     "fe_prefill_paged_window": (_i, [_p, _p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i,
                                      _f, _i, _i, _p, _sz, _p]),
     "fe_prefill_paged_kv4": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _p, _i, _i, _i, _i, _i,

@@ -223,6 +223,15 @@ extern "C" size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int 
   return b16 > b32 ? b16 : b32;
 }
 
+extern "C" int fe_span_prefill_rows(int num_seqs, int total_q, int num_q_heads, int kv_heads,
+                                    int head_dim, int window, int kv4, int elem_bytes) {
+  FE_CHECK_ARG(num_seqs > 0 && total_q > 0 && num_q_heads > 0 && kv_heads > 0 && head_dim > 0 &&
+               window >= 0 && num_q_heads % kv_heads == 0);
+  FE_CHECK_ARG(kv4 ? elem_bytes == 2 : (window > 0 && (elem_bytes == 2 || elem_bytes == 4)));
+  if (elem_bytes == 4) return kTile;
+  return 32 * span_waves(num_seqs, total_q, num_q_heads, kv_heads, head_dim, window, kv4 != 0);
+}
+
 #define FE_WINDOW_PREFILL(SUFFIX, E)                                                              \
   extern "C" int fe_prefill_paged_window##SUFFIX(                                                 \
       const void* q, void* out, const void* k_pool, const void* v_pool, int num_blocks,           \

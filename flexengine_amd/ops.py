@@ -791,6 +791,19 @@ def prefill_form(num_seqs: int, total_q: int, max_q_len: int, num_q_heads: int, 
     return _PREFILL_FORMS[rc]
 
 
+def span_prefill_rows(num_seqs: int, total_q: int, num_q_heads: int, kv_heads: int, head_dim: int,
+                      dtype: torch.dtype, *, window: int | None = None, sinks: int = 0,
+                      kv4: bool = False) -> int:
+    """Rows of a sequence that prefill_paged under a window or over 4-bit pools computes together
+    at these sizes (fe_span_prefill_rows): 16, 128 or 256."""
+    rows = _lib.load().fe_span_prefill_rows(num_seqs, total_q, num_q_heads, kv_heads, head_dim,
+                                            check_window(window, sinks)[0], int(kv4),
+                                            dtype.itemsize)
+    if rows < 0:
+        _lib.check("fe_span_prefill_rows", rows)
+    return rows
+
+
 def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                   block_tables: torch.Tensor, q_offsets: torch.Tensor,
                   context_lens: torch.Tensor, max_q_len: int, *, scale: float | None = None,

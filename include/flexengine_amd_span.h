@@ -160,8 +160,17 @@ size_t fe_span_prefill_workspace_size(int num_seqs, int total_q, int num_q_heads
                                       int head_dim);
 
 /*
+ * Rows (query heads of a KV head times positions) of a sequence that a prefill of these sizes
+ * computes together: 16 (elem_bytes 4), 128, or 256 (long prompts over 4-bit pools, kv4 != 0); a
+ * negative FE_ERR_* code for bad sizes.  Launches nothing; for tests and profiles.
+ */
+int fe_span_prefill_rows(int num_seqs, int total_q, int num_q_heads, int kv_heads, int head_dim,
+                         int window, int kv4, int elem_bytes);
+
+/*
  * fe_prefill_paged (flexengine_amd.h) under a window with sinks: the same rows, tables and
- * offsets, scale > 0.
+ * offsets, scale > 0.  A context past what the table addresses ends there; one of fewer tokens than
+ * its rows counts as just those rows.  No page past the table's last entry is read for it.
  */
 int fe_prefill_paged_window(const void* q, void* out, const void* k_pool, const void* v_pool,
                             int num_blocks, const int32_t* block_tables, int table_stride,
