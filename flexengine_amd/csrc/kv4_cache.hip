@@ -5,9 +5,9 @@
 // the magnitudes' bits), four conversions, one 4-byte store; the block's first thread stores
 // the scale.  The gather is the reverse.  A workgroup takes a run of tokens of kChunks such
 // chunks and looks their slots up first, one thread a token, over offsets and lengths in LDS:
-// looked up by every thread the chain of dependent loads was the kernels' length.  5900 tokens
-// of 8 heads of 128, 30 MB moved by each: write 10.8 -> 9.1 us, gather 10.1 -> 8.4 (of 6 at the
-// rate of a large copy; 2048 chunks a workgroup 12.2 and 10.9).
+// looked up by every thread the chain of dependent loads was the kernels' length.  6468 tokens
+// of 8 heads of 128, 33.5 MB moved by each: write 10.8 -> 9.1 us, gather 10.1 -> 8.4 (of 6.6 at
+// the rate of a large copy; 2048 chunks a workgroup 12.2 and 10.9).
 #include "kv4.h"
 #include "flexengine_amd_span.h"
 

@@ -16,7 +16,7 @@ namespace {
 // eight waves 50.5.  Units too few for the chip share their keys out over splits, as the 16-bit
 // kernel's do (span_prefill.h): 50 tokens over up to 3000 under a window of 2000 38.3 -> 15.7 us,
 // four chunks of 10-20 over up to 8000 under 4000 92.6 -> 35.8 (four chunks of 500 at head_dim 96,
-// not split, 128.5 -> 132 for its registers).
+// not split, 128.5 -> 132: that padded form spills 15 registers, 64 bytes of scratch a lane).
 constexpr int kF32Waves = 4;
 constexpr int kF32Slots = 768;  // workgroups that run at once: three on each of 256 CUs
 

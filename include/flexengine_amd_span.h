@@ -19,8 +19,8 @@
  * The _strided forms take the same dims in any order and with gaps between rows (fe_kv4_strides).
  * A write takes the smallest power of two 2^e with max|x| <= 7 * 2^e, -23 <= e <= 13 (fp16
  * rows) or 125 (bf16 rows), and rounds to the nearest code, ties to the even one.  Every value
- * is exact in the rows' type.  fp16 magnitudes above 49152 are held as 49152; a block with an
- * infinity or a NaN is held as NaN.  Two rows of one call in the same slot leave it undefined.
+ * is exact in the rows' type.  fp16 magnitudes above 49152 are held as 49152, a block (of either
+ * type) whose largest magnitude is at most 2^-25 as zeros; one with an infinity or a NaN as NaN.  Two rows of one call in the same slot leave it undefined.
  *
  * Shapes: block_size a power of two, of at least 16 for attention; head_dim a multiple of 32 up
  * to 256 (4-bit), a multiple of 8 up to 256 (fp16, bf16 windows) or up to 128 (fp32 windows);
