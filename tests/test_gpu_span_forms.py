@@ -8,7 +8,7 @@ import torch
 
 from flexengine_amd import ops
 from tests import span_ref as R
-from tests.test_gpu_span import BF16, DEV, F16, Pools, check_decode, gen
+from tests.test_gpu_span import BF16, DEV, F16, JUNK, Pools, check_decode, gen
 from tests.test_gpu_span_prefill import TYPES, Step
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +120,17 @@ def test_rows_past_the_table_leave_the_others_as_they_were(dt, bits):
     for a, b in ((0, 9), (49, 65), (65, 70)):
         assert torch.equal(got[a:b], full[a:b])
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dt,bits", TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 5)])
+def test_decode_behind_the_widest_table(dt, bits, window, sinks):
+    """Tables of 262144 tokens, as a captured step's may be, over contexts of at most 3000: the split
+    and the workspace are the table's, the entries past the contexts name no block."""
+    if bits != 4 and not window:
+        pytest.skip("the plain decode")
+    p = Pools([1, 3000, 0, 17, 64, 1500, 333], 16, 2, 128, dt, bits, window, sinks, 89)
+    wide = torch.full((7, 262144 // 16), JUNK, dtype=torch.int32, device=DEV)
+    wide[:, :p.tabs.shape[1]] = p.tabs
+    p.tabs = wide
+    check_decode(p, 12, 128, window or None, sinks, new=True)
